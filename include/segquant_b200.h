@@ -202,6 +202,55 @@ typedef struct sq_gated_residual_args {
 
 int sq_gated_residual(const sq_gated_residual_args* args, sq_stream_t stream);
 
+/* ---- attention (no counterpart in the reference, which calls torch's) --------------------------------------------
+ * out = softmax(scale * q k^T) v with the statistics in fp32, for 16-bit q, k, v, out of one type; Hq query heads share Hkv
+ * key heads evenly (query head h reads key head h / (Hq / Hkv)).  Two forms:
+ *   - sequences of one extent: q / out [batch, Tq, Hq, D], k / v [batch, Tk, Hkv, D]; q_lens_dev / kv_lens_dev (int32[batch], or
+ *     NULL) give the valid queries and keys of each (a padded batch, a cache that is not full), clamped to [0, Tq] / [0, Tk];
+ *   - packed: q / out [Tq, Hq, D], k / v [Tk, Hkv, D] with Tq / Tk tokens in all; sequence i has the tokens
+ *     [offsets[i], offsets[i + 1]) of each (int32[batch + 1], non-decreasing, clamped to the tensors).
+ * causal: query i of a sequence sees its keys [0, i + 1 + kv_len - q_len): the last query sits on the last key, so the
+ * queries of a prompt's next piece, or a single new token, continue the keys that are there.  A query that sees no key gets 0
+ * (lse: -inf).  Keys outside a sequence never reach its rows, whatever bits they hold; a NaN or infinity in a v row that
+ * another query of the sequence sees may also reach earlier queries (0 * inf), as in the product it stands for.
+ * Rows of out (and lse) that belong to no sequence are left alone, or set like rows that see no key with fill_rest.
+ * D: a multiple of 8 up to SQ_ATTENTION_MAX_D, contiguous; strides in elements, multiples of 8 and positive; pointers 16-byte
+ * aligned.  out must not overlap q, k or v.  lse_dev: NULL or float [tokens, Hq], log of the row sums (natural).
+ * scratch_dev: sq_attention_scratch_bytes(args) bytes (0 for most calls; few rows against many keys need some), 16-byte
+ * aligned, used by this call alone until the stream has run it.
+ */
+#define SQ_ATTENTION_MAX_D 128
+
+typedef struct sq_attention_args {
+    const void* q_dev;
+    const void* k_dev;
+    const void* v_dev;
+    void* out_dev;
+    float* lse_dev;
+    int32_t dtype;             /* SQ_F16 / SQ_BF16 */
+    int32_t causal;
+    int64_t batch, Tq, Tk;
+    int32_t Hq, Hkv, D;
+    int32_t fill_rest;
+    int64_t q_batch_stride, q_token_stride, q_head_stride;
+    int64_t k_batch_stride, k_token_stride, k_head_stride;
+    int64_t v_batch_stride, v_token_stride, v_head_stride;
+    int64_t out_batch_stride, out_token_stride, out_head_stride;
+    const int32_t* q_offsets_dev;
+    const int32_t* kv_offsets_dev;
+    const int32_t* q_lens_dev;
+    const int32_t* kv_lens_dev;
+    float scale;               /* > 0 */
+    int32_t reserved0;         /* must be 0 */
+    void* scratch_dev;
+    int64_t scratch_bytes;
+} sq_attention_args;
+
+int sq_attention(const sq_attention_args* args, sq_stream_t stream);
+/* Bytes of scratch that sq_attention needs for these arguments (pointers other than the offsets / lengths are not looked at),
+   or a negative status. */
+int64_t sq_attention_scratch_bytes(const sq_attention_args* args);
+
 /* ---- weight quantise / pack ---------------------------------------------------------------
  * Replaces real_quantized_quantize_weights<T> (real_gemm.cu:538-638; pybind names in
  * seg_utils.h:82-120).  w is [N, K] contiguous.  scale_mode 0: one scalar `scale_scalar`

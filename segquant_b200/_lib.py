@@ -9,6 +9,7 @@ import os
 SQ_MAX_SEGS = 64
 SQ_MAX_PEERS = 8
 SQ_STATIC_SCRATCH_BYTES = 64 * 1024 * 1024
+SQ_ATTENTION_MAX_D = 128
 
 SQ_OK = 0
 SQ_ERR_INVALID_ARG = -1
@@ -25,7 +26,7 @@ SQ_GEMM_W8A8_I8, SQ_GEMM_W8A8_F8, SQ_GEMM_W4A8 = 0, 1, 2
 
 EXPORTED_SYMBOLS = (
     "sq_version", "sq_last_error", "sq_status_string", "sq_device_status",
-    "sq_quantize_act", "sq_quantize_act_dynamic", "sq_norm_quantize_act", "sq_residual_norm_quantize_act", "sq_gated_residual", "sq_quantize_weight", "sq_unpack_int4",
+    "sq_quantize_act", "sq_quantize_act_dynamic", "sq_norm_quantize_act", "sq_residual_norm_quantize_act", "sq_gated_residual", "sq_attention", "sq_attention_scratch_bytes", "sq_quantize_weight", "sq_unpack_int4",
     "sq_gemm", "sq_gemm_num_units", "sq_seg_linear", "sq_seg_linear_static",
     "sq_check_device", "sq_set_wait_limit_cycles", "sq_wait_probe", "sq_set_gemm_schedule", "sq_push_columns", "sq_peer_barrier",
 )
@@ -72,6 +73,23 @@ class GatedResidualArgs(ctypes.Structure):
         ("y_batch_stride", ctypes.c_int64), ("y_row_stride", ctypes.c_int64),
         ("out_batch_stride", ctypes.c_int64), ("out_row_stride", ctypes.c_int64),
         ("gate_batch_stride", ctypes.c_int64),
+    ]
+
+
+class AttentionArgs(ctypes.Structure):
+    """struct sq_attention_args"""
+    _fields_ = [
+        ("q_dev", ctypes.c_void_p), ("k_dev", ctypes.c_void_p), ("v_dev", ctypes.c_void_p), ("out_dev", ctypes.c_void_p), ("lse_dev", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32), ("causal", ctypes.c_int32),
+        ("batch", ctypes.c_int64), ("Tq", ctypes.c_int64), ("Tk", ctypes.c_int64),
+        ("Hq", ctypes.c_int32), ("Hkv", ctypes.c_int32), ("D", ctypes.c_int32), ("fill_rest", ctypes.c_int32),
+        ("q_batch_stride", ctypes.c_int64), ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("k_batch_stride", ctypes.c_int64), ("k_token_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+        ("v_batch_stride", ctypes.c_int64), ("v_token_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64),
+        ("out_batch_stride", ctypes.c_int64), ("out_token_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64),
+        ("q_offsets_dev", ctypes.c_void_p), ("kv_offsets_dev", ctypes.c_void_p), ("q_lens_dev", ctypes.c_void_p), ("kv_lens_dev", ctypes.c_void_p),
+        ("scale", ctypes.c_float), ("reserved0", ctypes.c_int32),
+        ("scratch_dev", ctypes.c_void_p), ("scratch_bytes", ctypes.c_int64),
     ]
 
 
@@ -165,6 +183,10 @@ def load():
                                                   ctypes.c_float, ctypes.POINTER(NormResidual), ctypes.c_void_p]
     lib.sq_gated_residual.restype = ctypes.c_int
     lib.sq_gated_residual.argtypes = [ctypes.POINTER(GatedResidualArgs), ctypes.c_void_p]
+    lib.sq_attention.restype = ctypes.c_int
+    lib.sq_attention.argtypes = [ctypes.POINTER(AttentionArgs), ctypes.c_void_p]
+    lib.sq_attention_scratch_bytes.restype = ctypes.c_int64
+    lib.sq_attention_scratch_bytes.argtypes = [ctypes.POINTER(AttentionArgs)]
     lib.sq_norm_quantize_act.restype = ctypes.c_int
     lib.sq_norm_quantize_act.argtypes = [ctypes.POINTER(ActQuantArgs), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
                                          ctypes.c_float, ctypes.c_void_p]

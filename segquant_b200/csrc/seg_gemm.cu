@@ -18,7 +18,8 @@ static int g_last_tu = 0;   // (kind * 2 + dual) of the last launch; the trace r
 #define SQ_FOR_EACH_TU(X) X(SQ_GEMM_W8A8_I8, false) X(SQ_GEMM_W8A8_I8, true) X(SQ_GEMM_W8A8_F8, false) X(SQ_GEMM_W8A8_F8, true) \
                           X(SQ_GEMM_W4A8, false) X(SQ_GEMM_W4A8, true)
 
-long long push_read_status();   // peer_push.cu
+long long push_read_status();        // peer_push.cu
+long long attention_read_status();   // attention.cu
 
 long long read_device_status() {
     if (cudaDeviceSynchronize() != cudaSuccess) return SQ_ERR_CUDA;
@@ -33,6 +34,11 @@ long long read_device_status() {
 #undef SQ_X
     {
         const long long v = push_read_status();   // the peer barrier's word (peer_push.cu)
+        if (v < 0) return v;
+        if (first == 0) first = v;
+    }
+    {
+        const long long v = attention_read_status();
         if (v < 0) return v;
         if (first == 0) first = v;
     }
@@ -62,7 +68,7 @@ extern "C" int sq_trace_read(long long* out, int n) {
 // ---------------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------------
-static PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static bool tried = false;
     if (!tried) {
@@ -108,7 +114,7 @@ static int make_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t
         auto it = map_cache().find(key);
         if (it != map_cache().end()) { *map = it->second; return SQ_OK; }
     }
-    auto fn = get_encode_fn();
+    auto fn = tensor_map_encoder();
     SQ_REQUIRE(fn != nullptr, SQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
     cuuint64_t dims[3] = {inner, rows, batch};
     cuuint64_t strides[2] = {row_stride, batch_stride};

@@ -237,6 +237,119 @@ def quantize_act_dynamic(x, bounds, out_kind=L.SQ_Q_INT8, dual=False, smooth=Non
 
 
 # ---------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------
+def _no_grad(*tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("segquant_b200: this operator has no backward pass; detach its inputs or run it under torch.no_grad()")
+
+
+def _tma_view(t):
+    """t itself where the kernel can read it in place (last dimension contiguous, other strides positive multiples of 16
+    bytes, 16-byte aligned), else a contiguous copy."""
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
+    for n, s in zip(t.shape[:-1], t.stride()[:-1]):
+        ok = ok and (n <= 1 or (s > 0 and s % 8 == 0))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _int32_list(t, n, name, device):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or t.device != device:
+        raise ValueError(f"attention: {name} must be an int32 tensor of {n} elements on {device}")
+    return t.contiguous()
+
+
+def attention(q, k, v, *, causal=False, scale=None, q_offsets=None, kv_offsets=None, q_lens=None, kv_lens=None, out=None,
+              return_lse=False):
+    """softmax(scale * q k^T) v for 16-bit tensors, statistics in fp32; scale defaults to D ** -0.5.
+
+    Sequences of one extent: q (B, Tq, Hq, D), k and v (B, Tk, Hkv, D), Hq a multiple of Hkv (query head h reads key head
+    h // (Hq // Hkv)); q_lens / kv_lens (int32 (B,), on the device) give the valid tokens of each where they are fewer.
+    Packed sequences: q (Nq, Hq, D), k and v (Nk, Hkv, D) with q_offsets (int32 (B + 1,), non-decreasing, on the device);
+    kv_offsets defaults to q_offsets.  D is a multiple of 8 up to 128; strides are free as long as D is contiguous (views
+    that the loads cannot read in place are copied first).
+
+    causal: query i of a sequence sees its keys below i + 1 + kv_len - q_len, so its last query sees its last key.  A
+    query that sees no key gets 0 (lse -inf).  Rows that belong to no sequence are 0 in a new result and left alone in
+    `out`, which has q's shape and dtype, D contiguous, strides and address multiples of 16 bytes, and overlaps no input.
+    return_lse: also the float32 logarithm of the row sums, (B, Tq, Hq) or (Nq, Hq)."""
+    global launch_count
+    _need_cuda(q, k, v)
+    _no_grad(q, k, v)
+    packed = q_offsets is not None
+    if kv_offsets is not None and not packed:
+        raise ValueError("attention: kv_offsets needs q_offsets")
+    if packed and (q_lens is not None or kv_lens is not None):
+        raise ValueError("attention: packed sequences have offsets, not lengths")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("attention: q, k and v must share a 16-bit dtype")
+    rank = 3 if packed else 4
+    if q.dim() != rank or k.dim() != rank or v.shape != k.shape or k.shape[-1] != q.shape[-1] or (not packed and k.shape[0] != q.shape[0]):
+        raise ValueError("attention: q (B, Tq, Hq, D) with k, v (B, Tk, Hkv, D), or packed q (Nq, Hq, D) with k, v (Nk, Hkv, D)")
+    if k.device != q.device or v.device != q.device:
+        raise ValueError("attention: q, k and v must be on one device")
+    Tq, Hq, D = q.shape[-3:]
+    Tk, Hkv = k.shape[-3:-1]
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"attention: {Hq} query heads do not share {Hkv} key heads evenly")
+    if D % 8 or not 8 <= D <= L.SQ_ATTENTION_MAX_D:
+        raise ValueError(f"attention: head width {D} is not a multiple of 8 up to {L.SQ_ATTENTION_MAX_D}")
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError("attention: scale must be positive and finite")
+    a = L.AttentionArgs()
+    if packed:
+        kv_offsets = q_offsets if kv_offsets is None else kv_offsets
+        B = q_offsets.numel() - 1
+        if B < 0:
+            raise ValueError("attention: q_offsets needs at least one element")
+        q_offsets, kv_offsets = (_int32_list(t, B + 1, n, q.device) for t, n in ((q_offsets, "q_offsets"), (kv_offsets, "kv_offsets")))
+        a.q_offsets_dev, a.kv_offsets_dev = q_offsets.data_ptr(), kv_offsets.data_ptr()
+    else:
+        B = q.shape[0]
+        if q_lens is not None:
+            q_lens = _int32_list(q_lens, B, "q_lens", q.device)
+            a.q_lens_dev = q_lens.data_ptr()
+        if kv_lens is not None:
+            kv_lens = _int32_list(kv_lens, B, "kv_lens", q.device)
+            a.kv_lens_dev = kv_lens.data_ptr()
+    a.fill_rest = out is None
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _need_cuda(out)
+        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or _tma_view(out) is not out:
+            raise ValueError("attention: out must have q's shape, dtype and device, a contiguous last dimension, and strides and address in "
+                             "multiples of 16 bytes")
+    lse = torch.full(q.shape[:-1], float("-inf"), dtype=torch.float32, device=q.device) if return_lse else None
+    if packed and B == 0:
+        if a.fill_rest:
+            out.zero_()
+    elif q.numel():
+        q, k, v = _tma_view(q), _tma_view(k), _tma_view(v)
+        a.q_dev, a.k_dev, a.v_dev, a.out_dev = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+        a.lse_dev = lse.data_ptr() if return_lse else None
+        a.dtype, a.causal = _dt(q), 1 if causal else 0
+        a.batch, a.Tq, a.Tk, a.Hq, a.Hkv, a.D = B, Tq, Tk, Hq, Hkv, D
+        a.scale = scale
+        a.q_token_stride, a.q_head_stride = q.stride(-3), q.stride(-2)
+        a.k_token_stride, a.k_head_stride = k.stride(-3), k.stride(-2)
+        a.v_token_stride, a.v_head_stride = v.stride(-3), v.stride(-2)
+        a.out_token_stride, a.out_head_stride = out.stride(-3), out.stride(-2)
+        if not packed:
+            a.q_batch_stride, a.k_batch_stride, a.v_batch_stride, a.out_batch_stride = q.stride(0), k.stride(0), v.stride(0), out.stride(0)
+        lib = L.load()
+        need = L.check(lib.sq_attention_scratch_bytes(ctypes.byref(a)), "sq_attention_scratch_bytes")
+        scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        if need:
+            a.scratch_dev, a.scratch_bytes = scratch.data_ptr(), need
+        with torch.cuda.device(q.device):
+            L.check(lib.sq_attention(ctypes.byref(a), _stream(q)), "sq_attention")
+        launch_count += 2 if need else 1
+    return (out, lse) if return_lse else out
+
+
+# ---------------------------------------------------------------------------------------------
 # weights
 # ---------------------------------------------------------------------------------------------
 def quantize_weight(w, out, scale, out_kind, group_size=0):
