@@ -251,6 +251,47 @@ int sq_attention(const sq_attention_args* args, sq_stream_t stream);
    or a negative status. */
 int64_t sq_attention_scratch_bytes(const sq_attention_args* args);
 
+/* ---- rotary positions (no counterpart in the reference) -------------------------------------------------------------
+ * The D columns of a head are cut into one block of axes[a] columns per axis; columns behind the last block are not rotated.
+ * Pair i of axis a turns by  positions[b, t, a] * theta^(-2 i / axes[a])  (reduced in fp64):
+ *   (y0, y1) -> (y0 cos - y1 sin, y0 sin + y1 cos)
+ * with y = x, or with the norm weights y = x * rsqrt(mean(x^2) + eps) * weight over the head's D columns first.  Arithmetic in
+ * fp32, one rounding to the dtype of x.  Pairs are columns (2i, 2i + 1) of the block (SQ_ROTARY_ADJACENT) or (i, i + width / 2)
+ * (SQ_ROTARY_HALVES).  q is [batch, tokens, heads_q, D], k [batch, tokens, heads_k, D] (heads 0: absent), D contiguous, any
+ * other strides (elements); an out may be its input itself (same address and strides), but may not overlap it otherwise.
+ * positions: int32, or float32 with positions_float, the axes contiguous, pos_batch_stride 0 = shared by all batch entries.
+ * Multiples of 16 bytes (addresses, strides, D; for SQ_ROTARY_HALVES blocks of multiples of 16 columns) are the fast case.
+ */
+#define SQ_ROTARY_ADJACENT 0
+#define SQ_ROTARY_HALVES 1
+#define SQ_ROTARY_MAX_D 256
+#define SQ_ROTARY_MAX_AXES 8
+
+typedef struct sq_rotary_args {
+    const void* q_dev;
+    const void* k_dev;
+    void* q_out_dev;
+    void* k_out_dev;
+    int32_t dtype;             /* SQ_F32 / SQ_F16 / SQ_BF16 */
+    int32_t pairing;           /* SQ_ROTARY_* */
+    int64_t batch, tokens;
+    int32_t heads_q, heads_k, D, num_axes;
+    int32_t axes[SQ_ROTARY_MAX_AXES];
+    int64_t q_batch_stride, q_token_stride, q_head_stride;
+    int64_t k_batch_stride, k_token_stride, k_head_stride;
+    int64_t q_out_batch_stride, q_out_token_stride, q_out_head_stride;
+    int64_t k_out_batch_stride, k_out_token_stride, k_out_head_stride;
+    const void* positions_dev;
+    int64_t pos_batch_stride, pos_token_stride;
+    int32_t positions_float;
+    float eps;
+    double theta;
+    const void* norm_q_dev;    /* D weights in the dtype of x, or NULL: both or neither (where q and k are both there) */
+    const void* norm_k_dev;
+} sq_rotary_args;
+
+int sq_rotary(const sq_rotary_args* args, sq_stream_t stream);
+
 /* ---- weight quantise / pack ---------------------------------------------------------------
  * Replaces real_quantized_quantize_weights<T> (real_gemm.cu:538-638; pybind names in
  * seg_utils.h:82-120).  w is [N, K] contiguous.  scale_mode 0: one scalar `scale_scalar`

@@ -10,6 +10,8 @@ SQ_MAX_SEGS = 64
 SQ_MAX_PEERS = 8
 SQ_STATIC_SCRATCH_BYTES = 64 * 1024 * 1024
 SQ_ATTENTION_MAX_D = 128
+SQ_ROTARY_ADJACENT, SQ_ROTARY_HALVES = 0, 1
+SQ_ROTARY_MAX_D, SQ_ROTARY_MAX_AXES = 256, 8
 
 SQ_OK = 0
 SQ_ERR_INVALID_ARG = -1
@@ -26,7 +28,7 @@ SQ_GEMM_W8A8_I8, SQ_GEMM_W8A8_F8, SQ_GEMM_W4A8 = 0, 1, 2
 
 EXPORTED_SYMBOLS = (
     "sq_version", "sq_last_error", "sq_status_string", "sq_device_status",
-    "sq_quantize_act", "sq_quantize_act_dynamic", "sq_norm_quantize_act", "sq_residual_norm_quantize_act", "sq_gated_residual", "sq_attention", "sq_attention_scratch_bytes", "sq_quantize_weight", "sq_unpack_int4",
+    "sq_quantize_act", "sq_quantize_act_dynamic", "sq_norm_quantize_act", "sq_residual_norm_quantize_act", "sq_gated_residual", "sq_attention", "sq_attention_scratch_bytes", "sq_rotary", "sq_quantize_weight", "sq_unpack_int4",
     "sq_gemm", "sq_gemm_num_units", "sq_seg_linear", "sq_seg_linear_static",
     "sq_check_device", "sq_set_wait_limit_cycles", "sq_wait_probe", "sq_set_gemm_schedule", "sq_push_columns", "sq_peer_barrier",
 )
@@ -90,6 +92,25 @@ class AttentionArgs(ctypes.Structure):
         ("q_offsets_dev", ctypes.c_void_p), ("kv_offsets_dev", ctypes.c_void_p), ("q_lens_dev", ctypes.c_void_p), ("kv_lens_dev", ctypes.c_void_p),
         ("scale", ctypes.c_float), ("reserved0", ctypes.c_int32),
         ("scratch_dev", ctypes.c_void_p), ("scratch_bytes", ctypes.c_int64),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    """struct sq_rotary_args"""
+    _fields_ = [
+        ("q_dev", ctypes.c_void_p), ("k_dev", ctypes.c_void_p), ("q_out_dev", ctypes.c_void_p), ("k_out_dev", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32), ("pairing", ctypes.c_int32),
+        ("batch", ctypes.c_int64), ("tokens", ctypes.c_int64),
+        ("heads_q", ctypes.c_int32), ("heads_k", ctypes.c_int32), ("D", ctypes.c_int32), ("num_axes", ctypes.c_int32),
+        ("axes", ctypes.c_int32 * SQ_ROTARY_MAX_AXES),
+        ("q_batch_stride", ctypes.c_int64), ("q_token_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+        ("k_batch_stride", ctypes.c_int64), ("k_token_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64),
+        ("q_out_batch_stride", ctypes.c_int64), ("q_out_token_stride", ctypes.c_int64), ("q_out_head_stride", ctypes.c_int64),
+        ("k_out_batch_stride", ctypes.c_int64), ("k_out_token_stride", ctypes.c_int64), ("k_out_head_stride", ctypes.c_int64),
+        ("positions_dev", ctypes.c_void_p),
+        ("pos_batch_stride", ctypes.c_int64), ("pos_token_stride", ctypes.c_int64),
+        ("positions_float", ctypes.c_int32), ("eps", ctypes.c_float), ("theta", ctypes.c_double),
+        ("norm_q_dev", ctypes.c_void_p), ("norm_k_dev", ctypes.c_void_p),
     ]
 
 
@@ -183,6 +204,8 @@ def load():
                                                   ctypes.c_float, ctypes.POINTER(NormResidual), ctypes.c_void_p]
     lib.sq_gated_residual.restype = ctypes.c_int
     lib.sq_gated_residual.argtypes = [ctypes.POINTER(GatedResidualArgs), ctypes.c_void_p]
+    lib.sq_rotary.restype = ctypes.c_int
+    lib.sq_rotary.argtypes = [ctypes.POINTER(RotaryArgs), ctypes.c_void_p]
     lib.sq_attention.restype = ctypes.c_int
     lib.sq_attention.argtypes = [ctypes.POINTER(AttentionArgs), ctypes.c_void_p]
     lib.sq_attention_scratch_bytes.restype = ctypes.c_int64

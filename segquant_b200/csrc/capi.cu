@@ -27,6 +27,7 @@ int norm_quantize_act(const sq_act_quant_args* a, const void* shift, const void*
 int gated_residual(const sq_gated_residual_args* a, cudaStream_t st);
 int attention(const sq_attention_args* a, cudaStream_t st);
 long long attention_scratch_bytes(const sq_attention_args* a);
+int rotary(const sq_rotary_args* a, cudaStream_t st);
 int quantize_weight(const void* w, int w_dtype, long long N, long long K, int scale_mode, float scale_scalar,
                     const float* scale, int group_size, int out_kind, void* out, cudaStream_t st);
 int unpack_int4(const void* packed, void* out, long long numel, cudaStream_t st);
@@ -133,6 +134,11 @@ int sq_attention(const sq_attention_args* args, sq_stream_t stream) {
 int64_t sq_attention_scratch_bytes(const sq_attention_args* args) {
     sq::clear_error();
     return sq::attention_scratch_bytes(args);
+}
+
+int sq_rotary(const sq_rotary_args* args, sq_stream_t stream) {
+    sq::clear_error();
+    return sq::rotary(args, static_cast<cudaStream_t>(stream));
 }
 
 int sq_quantize_weight(const void* w_dev, int32_t w_dtype, int64_t N, int64_t K, int32_t scale_mode, float scale_scalar,

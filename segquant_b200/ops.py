@@ -237,6 +237,87 @@ def quantize_act_dynamic(x, bounds, out_kind=L.SQ_Q_INT8, dual=False, smooth=Non
 
 
 # ---------------------------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------------------------
+PAIRINGS = {"adjacent": L.SQ_ROTARY_ADJACENT, "halves": L.SQ_ROTARY_HALVES}
+
+
+def rotary(q, k, positions, axes, *, theta=10000.0, pairing="adjacent", norm_q=None, norm_k=None, eps=1e-6, out_q=None, out_k=None):
+    """Rotary positions with several axes on q (B, T, Hq, D) and k (B, T, Hk, D), or packed (N, H, D) ones; k may be None.
+
+    axes: the even widths of the axes' blocks inside a head, from column 0 on; columns behind the last block are not rotated.
+    positions: int32 or float32 (T, A) or (B, T, A) with A = len(axes) (packed: (N, A)).  Pair i of axis a turns by
+    position * theta ** (-2 i / axes[a]); pairing "adjacent" pairs columns (2i, 2i + 1) of a block, "halves" (i, i + width / 2).
+    norm_q / norm_k: (D,) weights of the heads' RMS normalisation in front of the rotation, in q's dtype, both or neither.
+    float32, float16 and bfloat16, D up to 256; arithmetic in fp32 (angles in fp64), rounded once.  out_q / out_k may be q / k
+    themselves.  Returns (q, k) rotated; (q, None) without k."""
+    global launch_count
+    _need_cuda(q, k, positions, norm_q, norm_k, out_q, out_k)
+    _no_grad(q, k, norm_q, norm_k)
+    if pairing not in PAIRINGS:
+        raise ValueError(f"pairing must be one of {list(PAIRINGS)}")
+    if q.dim() not in (3, 4) or (k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1])):
+        raise ValueError("rotary: q (B, T, Hq, D) and k (B, T, Hk, D), or packed (N, H, D) ones")
+    if k is not None and (k.dtype != q.dtype or k.device != q.device):
+        raise TypeError("rotary: q and k must share dtype and device")
+    if len(axes) == 0 or len(axes) > L.SQ_ROTARY_MAX_AXES:
+        raise ValueError(f"rotary: 1 to {L.SQ_ROTARY_MAX_AXES} axes")
+    B, T = (1, q.shape[0]) if q.dim() == 3 else q.shape[:2]
+    D = q.shape[-1]
+    want = (T, len(axes))
+    if tuple(positions.shape) != want and tuple(positions.shape) != (B, *want):
+        raise ValueError(f"rotary: positions must be {want} or {(B, *want)}, not {tuple(positions.shape)}")
+    if positions.dtype not in (torch.int32, torch.float32) or positions.device != q.device:
+        raise TypeError("rotary: positions must be int32 or float32 on q's device")
+    if k is not None and (norm_q is None) != (norm_k is None):
+        raise ValueError("rotary: norm_q and norm_k come together")
+    if k is None and norm_k is not None:
+        raise ValueError("rotary: norm_k without k")
+    for w in (norm_q, norm_k):
+        if w is not None and (tuple(w.shape) != (D,) or w.dtype != q.dtype or w.device != q.device):
+            raise ValueError("rotary: norm weights must be (D,) tensors of q's dtype on its device")
+    positions = positions.contiguous()
+    a = L.RotaryArgs()
+    a.dtype, a.pairing = _dt(q), PAIRINGS[pairing]
+    a.batch, a.tokens, a.D, a.num_axes = B, T, D, len(axes)
+    for i, w in enumerate(axes):
+        a.axes[i] = int(w)
+    a.positions_dev, a.positions_float = positions.data_ptr(), positions.dtype == torch.float32
+    a.pos_token_stride, a.pos_batch_stride = len(axes), (T * len(axes) if positions.dim() == 3 else 0)
+    a.eps, a.theta = float(eps), float(theta)
+    keep, outs = [], []
+    for name, x, out, w in (("q", q, out_q, norm_q), ("k", k, out_k, norm_k)):
+        if x is None:
+            if out is not None:
+                raise ValueError(f"rotary: out_{name} without {name}")
+            outs.append(None)
+            continue
+        if x.stride(-1) != 1:
+            if out is x:
+                raise ValueError("rotary: in place needs a contiguous last dimension")
+            x = x.contiguous()
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1:
+            raise ValueError(f"rotary: out_{name} must have {name}'s shape, dtype and device and a contiguous last dimension")
+        w = None if w is None else w.contiguous()
+        keep += [x, w]
+        outs.append(out)
+        setattr(a, "heads_" + name, x.shape[-2])
+        setattr(a, name + "_dev", x.data_ptr())
+        setattr(a, name + "_out_dev", out.data_ptr())
+        setattr(a, "norm_" + name + "_dev", None if w is None else w.data_ptr())
+        for pre, t in ((name, x), (name + "_out", out)):
+            setattr(a, pre + "_batch_stride", t.stride(0) if t.dim() == 4 else 0)
+            setattr(a, pre + "_token_stride", t.stride(-3))
+            setattr(a, pre + "_head_stride", t.stride(-2))
+    with torch.cuda.device(q.device):
+        L.check(L.load().sq_rotary(ctypes.byref(a), _stream(q)), "sq_rotary")
+    launch_count += 1
+    return tuple(outs)
+
+
+# ---------------------------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------------------------
 def _no_grad(*tensors):
