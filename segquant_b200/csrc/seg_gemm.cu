@@ -13,7 +13,7 @@ namespace sq {
 bool gemv_applies(const sq_gemm_args* a, bool dual);
 int launch_gemv(const GemmParams& p, const sq_gemm_args* a, bool dual, cudaStream_t st);
 // the same for packed int4 weights (seg_gemv_w4.cu)
-bool gemv_w4_applies(const sq_gemm_args* a, bool dual);
+bool gemv_w4_applies(const sq_gemm_args* a, bool dual, int units);
 int launch_gemv_w4(const GemmParams& p, const sq_gemm_args* a, bool dual, cudaStream_t st);
 
 static int g_last_tu = 0;   // (kind * 2 + dual) of the last launch; the trace reader of -DSQ_TRACE builds uses it
@@ -371,7 +371,7 @@ int gemm(const sq_gemm_args* a, cudaStream_t st) {
     p.wait_cycles = overrides().wait_cycles;
     // a handful of rows: stream the weights once on the CUDA cores instead of padding 128-row tensor-core tiles
     if (gemv_applies(a, dual)) return launch_gemv(p, a, dual, st);
-    if (gemv_w4_applies(a, dual)) return launch_gemv_w4(p, a, dual, st);
+    if (gemv_w4_applies(a, dual, units)) return launch_gemv_w4(p, a, dual, st);
     // Fused all-gather: stores to peers should be whole 128-byte lines ([16 rows x 128 bytes] boxes, see store_output).
     // That needs TMA-storable outputs and a tile whose per-warp column count is a multiple of the box (not 192 wide);
     // otherwise peers get the 16-column boxes of the plain store path.
