@@ -25,9 +25,20 @@ namespace sq {
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();   // seg_gemm.cu
 long long wait_limit_cycles();                            // seg_gemm.cu
 
-enum AttnWait : int { kAttnQ = 20, kAttnKvFull = 21, kAttnKvEmpty = 22, kAttnS = 23, kAttnSFree = 24, kAttnP = 25, kAttnPv = 26, kAttnTail = 27 };
+enum AttnWait : int { kAttnMma = 20, kAttnKvEmpty = 22, kAttnS = 23, kAttnPv = 26, kAttnTail = 27 };
 
 constexpr int kAttnThreads = 384;
+// Of kPolyOf pairs of exponentials, kPoly go to the FMA pipe (ex2_poly).  The special-function pipe does 4 lanes a cycle: two
+// warps' 128 exponentials a row take 2048 cycles there while everything else that a tile needs takes about 1000.
+#ifndef SQ_ATTN_POLY
+#define SQ_ATTN_POLY 1
+#define SQ_ATTN_POLY_OF 4
+#endif
+#ifndef SQ_ATTN_TURNS
+#define SQ_ATTN_TURNS 1
+#endif
+constexpr bool kTurns = SQ_ATTN_TURNS;
+constexpr int kPoly = SQ_ATTN_POLY, kPolyOf = SQ_ATTN_POLY_OF;
 constexpr int kAttnRows = 128;       // rows of a sub-tile = tensor-memory lanes
 constexpr int kAttnKeys = 128;       // keys of a tile
 
@@ -94,20 +105,21 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
         "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]));
 }
 
-// D (tensor memory, fp32) (+)= A (shared memory) B (shared memory), 16-bit operands of one type
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// D (tensor memory, fp32) (+)= A (shared memory) B (shared memory), 16-bit operands of one type.  Descriptors come as their
+// low words: the high word (layout, strides) is a constant.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kSmemDescHi)
         : "memory");
 }
 // the same with A in tensor memory
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kSmemDescHi)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait_all() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -250,80 +262,119 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             }
         } else if (warp == 9) {
             // ------------------------------------------------------------------ products
-            if (lane == 0 && n > 0) {
-                const uint32_t idesc_s = attn_idesc<T>(kAttnKeys, false);
-                const int dk = (p.D + 15) & ~15;
-                const uint32_t idesc_o = attn_idesc<T>(dk, true);
-                bool ok = true;
-                auto full = [&](int i) { return mbar_wait(smem_u32(&bar_full[i % ST]), (i / ST) & 1u, abort_flag, kAttnKvFull, p.wait_cycles); };
-                auto product_s = [&](int t, int j) {
-                    const uint32_t a = smem_desc_lo(q_smem(t)), b = smem_desc_lo(stage((2 * j) % ST));
-                    const int steps = dk >> 4;                 // 16 columns = 32 bytes each
-                    for (int k = 0; k < steps; ++k) {
+            // The whole warp walks the tiles in step (votes keep every address and branch uniform, so that the operands of the
+            // products are in uniform registers) and one lane issues.  With one lane walking alone an S took 460 cycles to issue
+            // and an O 590, and the issue, not the products, bounded the kernel: 3400 cycles for a pair of tiles.
+            uint32_t leader;
+            asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
+            const int n0 = __shfl_sync(0xffffffffu, n_sub[0], 0), n1 = __shfl_sync(0xffffffffu, n_sub[1], 0);
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), sb = __shfl_sync(0xffffffffu, sbase, 0);
+            const uint32_t idesc_s = attn_idesc<T>(kAttnKeys, false);
+            const int dk = (p.D + 15) & ~15;
+            const uint32_t idesc_o = attn_idesc<T>(dk, true);
+            bool ok = true;
+            auto wait_u = [&](uint32_t bar, uint32_t parity) {
+                if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return;
+                const long long t0 = clock64();
+                for (uint32_t it = 1; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++it) {
+                    if ((it & 1023u) == 0u && __any_sync(0xffffffffu, *abort_flag || clock64() - t0 > p.wait_cycles)) {
+                        if (leader) {
+                            if (!*abort_flag) wait_gave_up(kAttnMma);
+                            *abort_flag = 1;
+                        }
+                        ok = false;
+                        return;
+                    }
+                }
+            };
+            // K and V tiles lie in the ring in turn; the slot and the phase of the next K and of the next V of each sub-tile
+            auto full = [&](int i) { wait_u(smem_u32(&bar_full[i % ST]), (i / ST) & 1u); };
+            auto product_s = [&](int t, int j) {
+                const uint32_t a = smem_desc_lo(sb + t * C::kTile), b = smem_desc_lo(sb + (2 + (2 * j) % ST) * C::kTile);
+                if (leader) {
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {        // 16 columns = 32 bytes each
                         const uint32_t off = static_cast<uint32_t>(k >> 2) * (C::kHalf >> 4) + (k & 3) * 2u;
-                        mma_ss(tmem + C::col_s(t), smem_desc(a + off), smem_desc(b + off), idesc_s, k > 0);
+                        if (16 * k < dk) mma_ss(tm + C::col_s(t), a + off, b + off, idesc_s, k > 0);
                     }
                     umma_commit(smem_u32(&bar_s[t]));
-                };
-                auto product_o = [&](int t, int j) {
-                    // rows of 64 columns: 8 keys are 1024 bytes (SBO), the next 64 columns kHalf bytes on (LBO)
-                    const uint32_t b = ((stage((2 * j + 1) % ST) >> 4) & 0x3FFFu) | ((C::kHalf >> 4) << 16);
+                }
+            };
+            auto product_o = [&](int t, int j) {
+                // rows of 64 columns: 8 keys are 1024 bytes (SBO), the next 64 columns kHalf bytes on (LBO)
+                const uint32_t b = (((sb + (2 + (2 * j + 1) % ST) * C::kTile) >> 4) & 0x3FFFu) | ((C::kHalf >> 4) << 16);
+                const uint32_t first = j > 0;
+                if (leader) {
 #pragma unroll
                     for (int k = 0; k < kAttnKeys / 16; ++k)
-                        mma_ts(tmem + C::col_o(t), tmem + C::col_p(t) + k * 8, smem_desc(b + k * 128u), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+                        mma_ts(tm + C::col_o(t), tm + C::col_p(t) + k * 8, b + k * 128u, idesc_o, k > 0 ? 1u : first);
                     umma_commit(smem_u32(&bar_pv[t]));
-                };
-                auto wait_p = [&](int t, int j) {
-                    const bool r = mbar_wait(smem_u32(&bar_p[t]), j & 1u, abort_flag, kAttnP, p.wait_cycles);
+                }
+            };
+            auto release = [&](int i) {
+                if (leader) umma_commit(smem_u32(&bar_empty[i % ST]));
+            };
+            auto wait_p = [&](int t, int j) {
+                wait_u(smem_u32(&bar_p[t]), j & 1u);
+                tc_fence_after();
+            };
+            const int nn = n0 > n1 ? n0 : n1;
+            // S of tile 0
+            if (nn > 0) full(0);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                if (ok && (t ? n1 : n0) > 0) {
+                    wait_u(smem_u32(&bar_q[t]), 0u);
                     tc_fence_after();
-                    return r;
-                };
-                if constexpr (C::kOwnP) {
-                    for (int j = 0; ok && j <= n; ++j) {
-                        if (j < n) {
-                            if (!full(2 * j)) { ok = false; break; }
-                            for (int t = 0; t < 2; ++t) {
-                                if (j >= n_sub[t]) continue;
-                                if (j == 0) {
-                                    if (!mbar_wait(smem_u32(&bar_q[t]), 0, abort_flag, kAttnQ, p.wait_cycles)) { ok = false; break; }
-                                } else if (!mbar_wait(smem_u32(&bar_sfree[t]), (j - 1) & 1u, abort_flag, kAttnSFree, p.wait_cycles)) { ok = false; break; }
-                                tc_fence_after();
-                                product_s(t, j);
-                            }
-                            if (!ok) break;
-                            umma_commit(smem_u32(&bar_empty[(2 * j) % ST]));
-                        }
-                        if (j > 0) {
-                            if (!full(2 * j - 1)) { ok = false; break; }
-                            for (int t = 0; t < 2; ++t) {
-                                if (j - 1 >= n_sub[t]) continue;
-                                if (!wait_p(t, j - 1)) { ok = false; break; }
-                                product_o(t, j - 1);
-                            }
-                            if (!ok) break;
-                            umma_commit(smem_u32(&bar_empty[(2 * j - 1) % ST]));
-                        }
-                    }
-                } else {
-                    if (!full(0)) ok = false;
-                    for (int t = 0; ok && t < 2; ++t) {
-                        if (n_sub[t] == 0) continue;
-                        if (!mbar_wait(smem_u32(&bar_q[t]), 0, abort_flag, kAttnQ, p.wait_cycles)) { ok = false; break; }
+                    if (ok) product_s(t, 0);
+                }
+            if (nn > 0) release(0);
+            if constexpr (C::kOwnP) {
+                // in the order in which two sub-tiles half a tile apart get ready: S of 0, O of 1, S of 1, O of 0
+                for (int j = 0; ok && j <= nn; ++j) {
+                    const bool more = j + 1 < nn;
+                    if (more) full(2 * j + 2);
+                    if (ok && j + 1 < n0) {
+                        wait_u(smem_u32(&bar_sfree[0]), j & 1u);
                         tc_fence_after();
-                        product_s(t, 0);
+                        if (ok) product_s(0, j + 1);
                     }
-                    if (ok) umma_commit(smem_u32(&bar_empty[0]));
-                    for (int j = 0; ok && j < n; ++j) {
-                        if (!full(2 * j + 1) || (j + 1 < n && !full(2 * j + 2))) { ok = false; break; }
-                        for (int t = 0; t < 2; ++t) {
-                            if (j >= n_sub[t]) continue;
-                            if (!wait_p(t, j)) { ok = false; break; }
-                            product_o(t, j);
-                            if (j + 1 < n_sub[t]) product_s(t, j + 1);
+                    if (ok && j > 0) {
+                        if (j - 1 < n1) {
+                            if (j - 1 >= n0) full(2 * j - 1);
+                            if (ok) wait_p(1, j - 1);
+                            if (ok) product_o(1, j - 1);
                         }
-                        if (!ok) break;
-                        umma_commit(smem_u32(&bar_empty[(2 * j + 1) % ST]));
-                        if (j + 1 < n) umma_commit(smem_u32(&bar_empty[(2 * j + 2) % ST]));
+                        release(2 * j - 1);
+                    }
+                    if (ok && j + 1 < n1) {
+                        wait_u(smem_u32(&bar_sfree[1]), j & 1u);
+                        tc_fence_after();
+                        if (ok) product_s(1, j + 1);
+                    }
+                    if (ok && more) release(2 * j + 2);
+                    if (ok && j < n0) {
+                        full(2 * j + 1);
+                        if (ok) wait_p(0, j);
+                        if (ok) product_o(0, j);
+                    }
+                }
+            } else {
+                for (int j = 0; ok && j < nn; ++j) {
+                    const bool more = j + 1 < nn;
+                    full(2 * j + 1);
+                    if (ok && more) full(2 * j + 2);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (ok && j < (t ? n1 : n0)) {
+                            wait_p(t, j);
+                            if (ok) product_o(t, j);
+                            if (ok && j + 1 < (t ? n1 : n0)) product_s(t, j + 1);
+                        }
+                    }
+                    if (ok) {
+                        release(2 * j + 1);
+                        if (more) release(2 * j + 2);
                     }
                 }
             }
@@ -361,41 +412,64 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const int cols = (p.D + 15) & ~15;
         float m_ref = -INFINITY, l = 0.0f;
         bool ok = true;
-        for (int j = 0; j < nt; ++j) {
+        // The two warps of an SM quarter (one of each sub-tile) take turns with their exponentials: while one fills the
+        // special-function pipe the other loads, compares and stores.  A warp that gives up still passes its turns on.
+        const int turns = kTurns ? min(n_sub[0], n_sub[1]) : 0;
+        const int my_turn = 1 + t * 4 + (warp & 3), other_turn = 1 + (t ^ 1) * 4 + (warp & 3);
+        auto pass_turn = [&](int j) {
+            if (j + t < turns) asm volatile("bar.arrive %0, 64;" ::"r"(other_turn) : "memory");
+        };
+        if (t == 1 && turns > 0) asm volatile("bar.arrive %0, 64;" ::"r"(other_turn) : "memory");
+        int j = 0;
+        for (; j < nt; ++j) {
             if (!mbar_wait(bs, j & 1u, abort_flag, kAttnS, p.wait_cycles)) { ok = false; break; }
             tc_fence_after();
             uint32_t s[128];
+            const int key0 = (lo + j) * kAttnKeys;
+            const bool edge = key0 + kAttnKeys > seen_by_all;
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tmem_ld_x32(ts, s);
+            tmem_ld_x32(ts + 32, s + 32);
+            tmem_ld_wait_x32(s);
+            tmem_ld_wait_x32(s + 32);
+            tmem_ld_x32(ts + 64, s + 64);
+            tmem_ld_x32(ts + 96, s + 96);
+            if (edge) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_ld_x32(ts + i * 32, s + i * 32);
+                for (int i = 0; i < 64; ++i) s[i] = key0 + i < limit ? s[i] : 0xFF800000u;
+            }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_ld_wait_x32(s + i * 32);
+            for (int i = 0; i < 64; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+            tmem_ld_wait_x32(s + 64);
+            tmem_ld_wait_x32(s + 96);
             if constexpr (C::kOwnP) {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bsf);
             }
-            const int key0 = (lo + j) * kAttnKeys;
-            if (key0 + kAttnKeys > seen_by_all) {
+            if (edge) {
 #pragma unroll
-                for (int i = 0; i < 128; ++i) s[i] = key0 + i < limit ? s[i] : 0xFF800000u;
+                for (int i = 64; i < 128; ++i) s[i] = key0 + i < limit ? s[i] : 0xFF800000u;
             }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
+            for (int i = 64; i < 128; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
             const float m_new = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            // DP = 64: the product with the previous P is done before P (and, for a rescale, O) is touched
-            if constexpr (C::kOwnP) {
-                if (j > 0) {
-                    if (!mbar_wait(bpv, (j - 1) & 1u, abort_flag, kAttnPv, p.wait_cycles)) { ok = false; break; }
+            // DP = 64: the product with the previous P has to be done before P (and, for a rescale, O) is touched
+            bool pv_done = !C::kOwnP || j == 0;
+            auto wait_pv = [&]() {
+                if (!pv_done) {
+                    pv_done = true;
+                    if (!mbar_wait(bpv, (j - 1) & 1u, abort_flag, kAttnPv, p.wait_cycles)) ok = false;
                     tc_fence_after();
                 }
-            }
+            };
             const bool grow = (m_new - m_ref) * c > 8.0f;
             if (__any_sync(0xffffffffu, grow)) {
                 const float f = grow ? ex2((m_ref - m_new) * c) : 1.0f;
                 if (grow) m_ref = m_new;
                 l *= f;
                 if (j > 0) {
+                    wait_pv();
                     for (int i = 0; i < cols; i += 16) {
                         uint32_t o[16];
                         tmem_ld_x16(to + i, o);
@@ -406,6 +480,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     }
                 }
             }
+            if (j < turns) asm volatile("bar.sync %0, 64;" ::"r"(my_turn) : "memory");
             const float mc = m_ref == -INFINITY ? 0.0f : m_ref * c;
             const float2 c2 = make_float2(c, c), mc2 = make_float2(-mc, -mc);
             float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
@@ -413,27 +488,39 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
             for (int i = 0; i < 64; ++i) {
                 float2 e = __ffma2_rn(make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), c2, mc2);
-                e.x = ex2(e.x);
-                e.y = ex2(e.y);
+                if (i % kPolyOf < kPoly) {
+                    e = ex2_poly(e);
+                } else {
+                    e.x = ex2(e.x);
+                    e.y = ex2(e.y);
+                }
                 sum[i & 1] = __fadd2_rn(sum[i & 1], e);
                 pk[i] = pack2<T>(e.x, e.y);
-                if (i == 31) tmem_st_x32(tp, pk);
+                if (i == 31) {
+                    wait_pv();
+                    tmem_st_x32(tp, pk);
+                }
             }
+            pass_turn(j);
             tmem_st_x32(tp + 32, pk + 32);
             tmem_st_wait_all();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bp);
+            if (!ok) break;
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         }
+        if (!ok)
+            for (; j < turns; ++j) pass_turn(j);
         // ---- result
         if (ok && nt > 0) {
             ok = mbar_wait(bpv, (nt - 1) & 1u, abort_flag, kAttnPv, p.wait_cycles);
             tc_fence_after();
         }
         if (ok && live[t]) {
-            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-            const float lse2 = l > 0.0f || l != l ? m_ref * c + log2f(l) : -INFINITY;
+            const bool empty = m_ref == -INFINITY && l == l;     // no key seen (the polynomial's 2^-126 does not count)
+            const float inv = empty ? 0.0f : 1.0f / l;
+            const float lse2 = empty ? -INFINITY : m_ref * c + log2f(l);
             const long long token = static_cast<long long>(T0.b) * (p.q_off ? 0 : p.Tq) + T0.q_base + tok;
             const long long r = token * p.Hq + head;
             if (p.splits > 1) {
@@ -455,7 +542,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
                 if (!mine) continue;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = inv == 0.0f ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
+                for (int e = 0; e < 16; ++e) o[e] = empty ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
                 if (p.splits > 1) {
 #pragma unroll
                     for (int e = 0; e < 16; e += 4)
