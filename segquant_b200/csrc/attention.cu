@@ -30,15 +30,8 @@ enum AttnWait : int { kAttnMma = 20, kAttnKvEmpty = 22, kAttnS = 23, kAttnPv = 2
 constexpr int kAttnThreads = 384;
 // Of kPolyOf pairs of exponentials, kPoly go to the FMA pipe (ex2_poly).  The special-function pipe does 4 lanes a cycle: two
 // warps' 128 exponentials a row take 2048 cycles there while everything else that a tile needs takes about 1000.
-#ifndef SQ_ATTN_POLY
-#define SQ_ATTN_POLY 1
-#define SQ_ATTN_POLY_OF 4
-#endif
-#ifndef SQ_ATTN_TURNS
-#define SQ_ATTN_TURNS 1
-#endif
-constexpr bool kTurns = SQ_ATTN_TURNS;
-constexpr int kPoly = SQ_ATTN_POLY, kPolyOf = SQ_ATTN_POLY_OF;
+constexpr int kPoly = 1, kPolyOf = 4;
+constexpr int kWarpMma = 9;         // and the next one
 constexpr int kAttnRows = 128;       // rows of a sub-tile = tensor-memory lanes
 constexpr int kAttnKeys = 128;       // keys of a tile
 
@@ -189,7 +182,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             }
             for (int s = 0; s < ST; ++s) {
                 mbar_init(smem_u32(&bar_full[s]), 1);
-                mbar_init(smem_u32(&bar_empty[s]), 1);
+                mbar_init(smem_u32(&bar_empty[s]), C::kOwnP ? 2 : 1);      // arrivals of the warps that issue products
             }
             mbar_init(smem_u32(&bar_tail), 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -197,7 +190,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             prefetch_tmap(&map_k);
             prefetch_tmap(&map_v);
         }
-    } else if (warp == 9) {
+    } else if (warp == kWarpMma) {
         __syncwarp();
         tmem_alloc(smem_u32(&tmem_s), 512);
         tmem_relinquish();
@@ -237,7 +230,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     auto stage = [&](int s) { return sbase + (2 + s) * C::kTile; };
 
     if (warp >= 8) {
-        reg_dec<40>();
+        reg_dec<56>();
         if (warp == 8) {
             // ------------------------------------------------------------------ loads
             if (lane == 0 && n > 0) {
@@ -260,125 +253,133 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                         tma_load_4d(stage(s) + h * C::kHalf, is_v ? &map_v : &map_k, h * 64, kvh, T0.kv_base + (lo + j) * kAttnKeys, T0.b, bar);
                 }
             }
-        } else if (warp == 9) {
+        } else if (warp == kWarpMma || warp == kWarpMma + 1) {
             // ------------------------------------------------------------------ products
-            // The whole warp walks the tiles in step (votes keep every address and branch uniform, so that the operands of the
-            // products are in uniform registers) and one lane issues.  With one lane walking alone an S took 460 cycles to issue
-            // and an O 590, and the issue, not the products, bounded the kernel: 3400 cycles for a pair of tiles.
+            // A warp alone takes 5 cycles an instruction, 80 to get past a barrier that is complete and 40 to issue a product (that
+            // runs for 32 to 64).  The whole warp walks in step (votes and shuffles keep branches and addresses uniform, so that the
+            // operands are in uniform registers) and one lane issues: with a lane walking alone an S took 460 cycles to issue and an O
+            // 590.  DP = 64 has a warp for each sub-tile: one for both needed 2100 cycles a pair of tiles, which bounded the kernel,
+            // for products that take 1100.  DP = 128, where the products take 2048 and S waits for O, has one warp for both: two were
+            // measured 10 % slower (12288 tokens, causal: 552 against 499 us), their products of one sub-tile wait behind the other's.
             uint32_t leader;
             asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leader));
             const int n0 = __shfl_sync(0xffffffffu, n_sub[0], 0), n1 = __shfl_sync(0xffffffffu, n_sub[1], 0);
+            const int nn = n0 > n1 ? n0 : n1;
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), sb = __shfl_sync(0xffffffffu, sbase, 0);
-            const uint32_t idesc_s = attn_idesc<T>(kAttnKeys, false);
             const int dk = (p.D + 15) & ~15;
-            const uint32_t idesc_o = attn_idesc<T>(dk, true);
+            const uint32_t idesc_s = attn_idesc<T>(kAttnKeys, false), idesc_o = attn_idesc<T>(dk, true);
+            const uint32_t b_full = smem_u32(&bar_full[0]), b_empty = smem_u32(&bar_empty[0]), b_q = smem_u32(&bar_q[0]), b_s = smem_u32(&bar_s[0]),
+                           b_sfree = smem_u32(&bar_sfree[0]), b_p = smem_u32(&bar_p[0]), b_pv = smem_u32(&bar_pv[0]);
             bool ok = true;
-            auto wait_u = [&](uint32_t bar, uint32_t parity) {
-                if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return;
-                const long long t0 = clock64();
-                for (uint32_t it = 1; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++it) {
-                    if ((it & 1023u) == 0u && __any_sync(0xffffffffu, *abort_flag || clock64() - t0 > p.wait_cycles)) {
-                        if (leader) {
-                            if (!*abort_flag) wait_gave_up(kAttnMma);
-                            *abort_flag = 1;
+            // two barriers at once: one round trip
+            auto wait2 = [&](uint32_t bar_a, uint32_t par_a, uint32_t bar_b, uint32_t par_b) {
+                if (!ok) return;
+                uint32_t it = 0;
+                long long t0 = 0;
+                for (;;) {
+                    const uint32_t ra = mbar_try_wait(bar_a, par_a), rb = mbar_try_wait(bar_b, par_b);
+                    if (__all_sync(0xffffffffu, ra & rb)) break;
+                    if ((it++ & 1023u) == 0u) {
+                        if (it == 1u) t0 = clock64();
+                        if (__any_sync(0xffffffffu, *abort_flag || clock64() - t0 > p.wait_cycles)) {
+                            if (leader) {
+                                if (!*abort_flag) wait_gave_up(kAttnMma);
+                                *abort_flag = 1;
+                            }
+                            ok = false;
+                            return;
                         }
-                        ok = false;
-                        return;
                     }
                 }
-            };
-            // K and V tiles lie in the ring in turn; the slot and the phase of the next K and of the next V of each sub-tile
-            auto full = [&](int i) { wait_u(smem_u32(&bar_full[i % ST]), (i / ST) & 1u); };
-            auto product_s = [&](int t, int j) {
-                const uint32_t a = smem_desc_lo(sb + t * C::kTile), b = smem_desc_lo(sb + (2 + (2 * j) % ST) * C::kTile);
-                if (leader) {
-#pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) {        // 16 columns = 32 bytes each
-                        const uint32_t off = static_cast<uint32_t>(k >> 2) * (C::kHalf >> 4) + (k & 3) * 2u;
-                        if (16 * k < dk) mma_ss(tm + C::col_s(t), a + off, b + off, idesc_s, k > 0);
-                    }
-                    umma_commit(smem_u32(&bar_s[t]));
-                }
-            };
-            auto product_o = [&](int t, int j) {
-                // rows of 64 columns: 8 keys are 1024 bytes (SBO), the next 64 columns kHalf bytes on (LBO)
-                const uint32_t b = (((sb + (2 + (2 * j + 1) % ST) * C::kTile) >> 4) & 0x3FFFu) | ((C::kHalf >> 4) << 16);
-                const uint32_t first = j > 0;
-                if (leader) {
-#pragma unroll
-                    for (int k = 0; k < kAttnKeys / 16; ++k)
-                        mma_ts(tm + C::col_o(t), tm + C::col_p(t) + k * 8, b + k * 128u, idesc_o, k > 0 ? 1u : first);
-                    umma_commit(smem_u32(&bar_pv[t]));
-                }
-            };
-            auto release = [&](int i) {
-                if (leader) umma_commit(smem_u32(&bar_empty[i % ST]));
-            };
-            auto wait_p = [&](int t, int j) {
-                wait_u(smem_u32(&bar_p[t]), j & 1u);
                 tc_fence_after();
             };
-            const int nn = n0 > n1 ? n0 : n1;
-            // S of tile 0
-            if (nn > 0) full(0);
+            auto wait1 = [&](uint32_t bar, uint32_t par) { wait2(bar, par, bar, par); };
+            // ring slot and lap of the next K and the next V tile (K and V lie in it in turn)
+            int ks = 0, kl = 0, vs = 1, vl = 0;
+            auto next_k = [&]() {
+                ks += 2;
+                if (ks >= ST) { ks -= ST; kl ^= 1; }
+            };
+            auto next_v = [&]() {
+                vs += 2;
+                if (vs >= ST) { vs -= ST; vl ^= 1; }
+            };
+            auto product_s = [&](int t, bool release) {
+                const uint32_t a = smem_desc_lo(sb + t * C::kTile), b = smem_desc_lo(sb + (2 + ks) * C::kTile), d = tm + C::col_s(0) + t * (C::col_s(1) - C::col_s(0));
+                if (leader) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-                if (ok && (t ? n1 : n0) > 0) {
-                    wait_u(smem_u32(&bar_q[t]), 0u);
-                    tc_fence_after();
-                    if (ok) product_s(t, 0);
+                    for (int k = 0; k < DP / 16; ++k) {            // 16 columns = 32 bytes each
+                        const uint32_t off = static_cast<uint32_t>(k >> 2) * (C::kHalf >> 4) + (k & 3) * 2u;
+                        if (16 * k < dk) mma_ss(d, a + off, b + off, idesc_s, k > 0);
+                    }
+                    umma_commit(b_s + t * 8);
+                    if (release) umma_commit(b_empty + ks * 8);
                 }
-            if (nn > 0) release(0);
+            };
+            auto product_o = [&](int t, uint32_t acc, bool release) {
+                // rows of 64 columns: 8 keys are 1024 bytes (SBO), the next 64 columns kHalf bytes on (LBO)
+                const uint32_t b = (((sb + (2 + vs) * C::kTile) >> 4) & 0x3FFFu) | ((C::kHalf >> 4) << 16), a = tm + C::col_p(0) + t * (C::col_p(1) - C::col_p(0)),
+                               d = tm + C::col_o(0) + t * (C::col_o(1) - C::col_o(0));
+                if (leader) {
+#pragma unroll
+                    for (int k = 0; k < kAttnKeys / 16; ++k) mma_ts(d, a + k * 8, b + k * 128u, idesc_o, k > 0 ? 1u : acc);
+                    umma_commit(b_pv + t * 8);
+                    if (release) umma_commit(b_empty + vs * 8);
+                }
+            };
             if constexpr (C::kOwnP) {
-                // in the order in which two sub-tiles half a tile apart get ready: S of 0, O of 1, S of 1, O of 0
-                for (int j = 0; ok && j <= nn; ++j) {
-                    const bool more = j + 1 < nn;
-                    if (more) full(2 * j + 2);
-                    if (ok && j + 1 < n0) {
-                        wait_u(smem_u32(&bar_sfree[0]), j & 1u);
-                        tc_fence_after();
-                        if (ok) product_s(0, j + 1);
-                    }
-                    if (ok && j > 0) {
-                        if (j - 1 < n1) {
-                            if (j - 1 >= n0) full(2 * j - 1);
-                            if (ok) wait_p(1, j - 1);
-                            if (ok) product_o(1, j - 1);
-                        }
-                        release(2 * j - 1);
-                    }
-                    if (ok && j + 1 < n1) {
-                        wait_u(smem_u32(&bar_sfree[1]), j & 1u);
-                        tc_fence_after();
-                        if (ok) product_s(1, j + 1);
-                    }
-                    if (ok && more) release(2 * j + 2);
-                    if (ok && j < n0) {
-                        full(2 * j + 1);
-                        if (ok) wait_p(0, j);
-                        if (ok) product_o(0, j);
-                    }
+                const int t = warp - kWarpMma, nt = t ? n1 : n0;
+                if (nt > 0) {
+                    wait2(b_full, 0u, b_q + t * 8, 0u);
+                    if (ok) product_s(t, true);
+                    next_k();
                 }
-            } else {
+                for (int j = 0; ok && j < nt; ++j) {
+                    if (j + 1 < nt) {
+                        wait2(b_full + ks * 8, kl, b_sfree + t * 8, j & 1u);
+                        if (ok) product_s(t, true);
+                        next_k();
+                    }
+                    wait2(b_full + vs * 8, vl, b_p + t * 8, j & 1u);
+                    if (ok) product_o(t, j > 0, true);
+                    next_v();
+                }
+                // tiles that only the other sub-tile needs: released as they come
+                for (int i = 2 * nt; ok && i < 2 * nn; ++i) {
+                    const int lap = i / ST, s = i - lap * ST;
+                    wait1(b_full + s * 8, lap & 1u);
+                    if (ok && leader) mbar_arrive(b_empty + s * 8);
+                }
+            } else if (warp == kWarpMma) {
+                // O of tile j and S of tile j + 1 of sub-tile 0, then of sub-tile 1; whichever comes last gives the slots back
+                if (nn > 0) {
+                    wait1(b_full, 0u);
+                    for (int t = 0; t < 2; ++t)
+                        if ((t ? n1 : n0) > 0) {
+                            wait1(b_q + t * 8, 0u);
+                            if (ok) product_s(t, t == 1 || n1 == 0);
+                        }
+                    next_k();
+                }
                 for (int j = 0; ok && j < nn; ++j) {
                     const bool more = j + 1 < nn;
-                    full(2 * j + 1);
-                    if (ok && more) full(2 * j + 2);
+                    const int kb = more ? ks : vs, kp = more ? kl : vl;
+                    wait2(b_full + vs * 8, vl, b_full + kb * 8, kp);
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        if (ok && j < (t ? n1 : n0)) {
-                            wait_p(t, j);
-                            if (ok) product_o(t, j);
-                            if (ok && j + 1 < (t ? n1 : n0)) product_s(t, j + 1);
+                        const int nt = t ? n1 : n0;
+                        if (ok && j < nt) {
+                            wait1(b_p + t * 8, j & 1u);
+                            if (ok) product_o(t, j > 0, t == 1 || j >= n1);
+                            if (ok && j + 1 < nt) product_s(t, t == 1 || j + 1 >= n1);
                         }
                     }
-                    if (ok) {
-                        release(2 * j + 1);
-                        if (more) release(2 * j + 2);
-                    }
+                    if (more) next_k();
+                    next_v();
                 }
             }
-        } else if (warp == 10 && tail) {
+            __syncwarp();
+        } else if (warp == kWarpMma + 2 && tail) {
             // ------------------------------------------------------------------ rows behind the last key
             const int s = (2 * n - 1) % ST;
             if (mbar_wait(smem_u32(&bar_tail), 0, abort_flag, kAttnTail, p.wait_cycles)) {
@@ -394,7 +395,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
     } else {
         // ---------------------------------------------------------------------- softmax
-        reg_inc<224>();
+        reg_inc<216>();
         const int t = warp >> 2;
         const int row = threadIdx.x & 127;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
@@ -414,7 +415,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         bool ok = true;
         // The two warps of an SM quarter (one of each sub-tile) take turns with their exponentials: while one fills the
         // special-function pipe the other loads, compares and stores.  A warp that gives up still passes its turns on.
-        const int turns = kTurns ? min(n_sub[0], n_sub[1]) : 0;
+        const int turns = min(n_sub[0], n_sub[1]);
         const int my_turn = 1 + t * 4 + (warp & 3), other_turn = 1 + (t ^ 1) * 4 + (warp & 3);
         auto pass_turn = [&](int j) {
             if (j + t < turns) asm volatile("bar.arrive %0, 64;" ::"r"(other_turn) : "memory");
@@ -507,7 +508,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bp);
-            if (!ok) break;
+            if (!ok) { ++j; break; }                               // this tile's turn has been passed on
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         }
         if (!ok)
@@ -570,7 +571,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kWarpMma) {
         __syncwarp();
         tc_fence_after();
         tmem_dealloc(tmem, 512);
