@@ -24,11 +24,26 @@ KERNELS = {
     "Wint4Aint8": (L.SQ_GEMM_W4A8, L.SQ_Q_INT8, L.SQ_Q_INT4),
 }
 
+_Bounds = ctypes.c_int32 * (L.SQ_MAX_SEGS + 1)
+
 launch_count = 0  # kernels of this library launched by this process (bench.py reports it)
 
 
 def _stream(t):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+def _run(fn, what, t, *args):
+    """Calls a C entry point with the current stream of t's device (made current for the call if it is not) and checks its status.
+    Spelled out without context managers where it can be: a small operator is done before its Python call returns."""
+    dev = t.get_device()
+    if torch.cuda.current_device() == dev:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if status < 0:
+        L.check(status, what)
 
 
 def _need_cuda(*tensors):
@@ -239,6 +254,7 @@ def quantize_act_dynamic(x, bounds, out_kind=L.SQ_Q_INT8, dual=False, smooth=Non
 # ---------------------------------------------------------------------------------------------
 # rotary positions
 # ---------------------------------------------------------------------------------------------
+_Axes = ctypes.c_int32 * L.SQ_ROTARY_MAX_AXES
 PAIRINGS = {"adjacent": L.SQ_ROTARY_ADJACENT, "halves": L.SQ_ROTARY_HALVES}
 
 
@@ -256,17 +272,17 @@ def rotary(q, k, positions, axes, *, theta=10000.0, pairing="adjacent", norm_q=N
     _no_grad(q, k, norm_q, norm_k)
     if pairing not in PAIRINGS:
         raise ValueError(f"pairing must be one of {list(PAIRINGS)}")
-    if q.dim() not in (3, 4) or (k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1])):
+    qs, dt = q.shape, q.dtype
+    if len(qs) not in (3, 4) or (k is not None and (k.shape[:-2] != qs[:-2] or k.shape[-1] != qs[-1])):
         raise ValueError("rotary: q (B, T, Hq, D) and k (B, T, Hk, D), or packed (N, H, D) ones")
-    if k is not None and (k.dtype != q.dtype or k.device != q.device):
+    if k is not None and (k.dtype != dt or k.device != q.device):
         raise TypeError("rotary: q and k must share dtype and device")
     if len(axes) == 0 or len(axes) > L.SQ_ROTARY_MAX_AXES:
         raise ValueError(f"rotary: 1 to {L.SQ_ROTARY_MAX_AXES} axes")
-    B, T = (1, q.shape[0]) if q.dim() == 3 else q.shape[:2]
-    D = q.shape[-1]
-    want = (T, len(axes))
-    if tuple(positions.shape) != want and tuple(positions.shape) != (B, *want):
-        raise ValueError(f"rotary: positions must be {want} or {(B, *want)}, not {tuple(positions.shape)}")
+    B, T = (1, qs[0]) if len(qs) == 3 else qs[:2]
+    D = qs[-1]
+    if positions.shape[-2:] != (T, len(axes)) or (positions.dim() != 2 and tuple(positions.shape) != (B, T, len(axes))):
+        raise ValueError(f"rotary: positions must be {(T, len(axes))} or {(B, T, len(axes))}, not {tuple(positions.shape)}")
     if positions.dtype not in (torch.int32, torch.float32) or positions.device != q.device:
         raise TypeError("rotary: positions must be int32 or float32 on q's device")
     if k is not None and (norm_q is None) != (norm_k is None):
@@ -274,46 +290,48 @@ def rotary(q, k, positions, axes, *, theta=10000.0, pairing="adjacent", norm_q=N
     if k is None and norm_k is not None:
         raise ValueError("rotary: norm_k without k")
     for w in (norm_q, norm_k):
-        if w is not None and (tuple(w.shape) != (D,) or w.dtype != q.dtype or w.device != q.device):
+        if w is not None and (w.shape != (D,) or w.dtype != dt or w.device != q.device):
             raise ValueError("rotary: norm weights must be (D,) tensors of q's dtype on its device")
     positions = positions.contiguous()
-    a = L.RotaryArgs()
-    a.dtype, a.pairing = _dt(q), PAIRINGS[pairing]
-    a.batch, a.tokens, a.D, a.num_axes = B, T, D, len(axes)
-    for i, w in enumerate(axes):
-        a.axes[i] = int(w)
-    a.positions_dev, a.positions_float = positions.data_ptr(), positions.dtype == torch.float32
-    a.pos_token_stride, a.pos_batch_stride = len(axes), (T * len(axes) if positions.dim() == 3 else 0)
-    a.eps, a.theta = float(eps), float(theta)
-    keep, outs = [], []
+    keep, outs, ptrs, out_ptrs, heads, strides, out_strides, norms = [], [], [], [], [], [], [], []
     for name, x, out, w in (("q", q, out_q, norm_q), ("k", k, out_k, norm_k)):
         if x is None:
             if out is not None:
                 raise ValueError(f"rotary: out_{name} without {name}")
             outs.append(None)
+            ptrs.append(None)
+            out_ptrs.append(None)
+            norms.append(None)
+            heads.append(0)
+            strides += (0, 0, 0)
+            out_strides += (0, 0, 0)
             continue
         if x.stride(-1) != 1:
             if out is x:
                 raise ValueError("rotary: in place needs a contiguous last dimension")
             x = x.contiguous()
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1:
+            out = torch.empty(x.shape, dtype=dt, device=x.device)
+        elif out.shape != x.shape or out.dtype != dt or out.device != x.device or out.stride(-1) != 1:
             raise ValueError(f"rotary: out_{name} must have {name}'s shape, dtype and device and a contiguous last dimension")
         w = None if w is None else w.contiguous()
-        keep += [x, w]
+        keep += (x, w)
         outs.append(out)
-        setattr(a, "heads_" + name, x.shape[-2])
-        setattr(a, name + "_dev", x.data_ptr())
-        setattr(a, name + "_out_dev", out.data_ptr())
-        setattr(a, "norm_" + name + "_dev", None if w is None else w.data_ptr())
-        for pre, t in ((name, x), (name + "_out", out)):
-            setattr(a, pre + "_batch_stride", t.stride(0) if t.dim() == 4 else 0)
-            setattr(a, pre + "_token_stride", t.stride(-3))
-            setattr(a, pre + "_head_stride", t.stride(-2))
-    with torch.cuda.device(q.device):
-        L.check(L.load().sq_rotary(ctypes.byref(a), _stream(q)), "sq_rotary")
-    launch_count += 1
+        ptrs.append(x.data_ptr())
+        out_ptrs.append(out.data_ptr())
+        norms.append(None if w is None else w.data_ptr())
+        heads.append(x.shape[-2])
+        for t, into in ((x, strides), (out, out_strides)):
+            st = t.stride()
+            into += st[:3] if len(st) == 4 else (0, *st[:2])
+    A = len(axes)
+    a = L.RotaryArgs(
+        ptrs[0], ptrs[1], out_ptrs[0], out_ptrs[1], _dt(q), PAIRINGS[pairing], B, T, heads[0], heads[1], D, A, _Axes(*axes),
+        *strides, *out_strides, positions.data_ptr(), T * A if positions.dim() == 3 else 0, A,
+        1 if positions.dtype == torch.float32 else 0, eps, theta, norms[0], norms[1])
+    _run(L.load().sq_rotary, "sq_rotary", q, ctypes.byref(a))
+    if B * T * (heads[0] + heads[1]):
+        launch_count += 1
     return tuple(outs)
 
 
@@ -328,10 +346,11 @@ def _no_grad(*tensors):
 def _tma_view(t):
     """t itself where the kernel can read it in place (last dimension contiguous, other strides positive multiples of 16
     bytes, 16-byte aligned), else a contiguous copy."""
-    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0
-    for n, s in zip(t.shape[:-1], t.stride()[:-1]):
-        ok = ok and (n <= 1 or (s > 0 and s % 8 == 0))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+    st = t.stride()
+    if st[-1] == 1 and t.data_ptr() % 16 == 0 and (t.is_contiguous() and st[-2] % 8 == 0 or
+                                                   all(n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:-1], st[:-1]))):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _int32_list(t, n, name, device):
@@ -362,15 +381,16 @@ def attention(q, k, v, *, causal=False, scale=None, q_offsets=None, kv_offsets=N
         raise ValueError("attention: kv_offsets needs q_offsets")
     if packed and (q_lens is not None or kv_lens is not None):
         raise ValueError("attention: packed sequences have offsets, not lengths")
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+    dt, qs, ks = q.dtype, q.shape, k.shape
+    if dt not in (torch.bfloat16, torch.float16) or k.dtype != dt or v.dtype != dt:
         raise TypeError("attention: q, k and v must share a 16-bit dtype")
     rank = 3 if packed else 4
-    if q.dim() != rank or k.dim() != rank or v.shape != k.shape or k.shape[-1] != q.shape[-1] or (not packed and k.shape[0] != q.shape[0]):
+    if len(qs) != rank or len(ks) != rank or v.shape != ks or ks[-1] != qs[-1] or (not packed and ks[0] != qs[0]):
         raise ValueError("attention: q (B, Tq, Hq, D) with k, v (B, Tk, Hkv, D), or packed q (Nq, Hq, D) with k, v (Nk, Hkv, D)")
     if k.device != q.device or v.device != q.device:
         raise ValueError("attention: q, k and v must be on one device")
-    Tq, Hq, D = q.shape[-3:]
-    Tk, Hkv = k.shape[-3:-1]
+    Tq, Hq, D = qs[-3:]
+    Tk, Hkv = ks[-3:-1]
     if Hkv == 0 or Hq % Hkv:
         raise ValueError(f"attention: {Hq} query heads do not share {Hkv} key heads evenly")
     if D % 8 or not 8 <= D <= L.SQ_ATTENTION_MAX_D:
@@ -378,54 +398,49 @@ def attention(q, k, v, *, causal=False, scale=None, q_offsets=None, kv_offsets=N
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError("attention: scale must be positive and finite")
-    a = L.AttentionArgs()
     if packed:
         kv_offsets = q_offsets if kv_offsets is None else kv_offsets
         B = q_offsets.numel() - 1
         if B < 0:
             raise ValueError("attention: q_offsets needs at least one element")
-        q_offsets, kv_offsets = (_int32_list(t, B + 1, n, q.device) for t, n in ((q_offsets, "q_offsets"), (kv_offsets, "kv_offsets")))
-        a.q_offsets_dev, a.kv_offsets_dev = q_offsets.data_ptr(), kv_offsets.data_ptr()
+        q_offsets, kv_offsets = _int32_list(q_offsets, B + 1, "q_offsets", q.device), _int32_list(kv_offsets, B + 1, "kv_offsets", q.device)
     else:
-        B = q.shape[0]
+        B = qs[0]
         if q_lens is not None:
             q_lens = _int32_list(q_lens, B, "q_lens", q.device)
-            a.q_lens_dev = q_lens.data_ptr()
         if kv_lens is not None:
             kv_lens = _int32_list(kv_lens, B, "kv_lens", q.device)
-            a.kv_lens_dev = kv_lens.data_ptr()
-    a.fill_rest = out is None
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    fill_rest = out is None
+    if fill_rest:
+        out = torch.empty(qs, dtype=dt, device=q.device)
     else:
         _need_cuda(out)
-        if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or _tma_view(out) is not out:
+        if out.shape != qs or out.dtype != dt or out.device != q.device or _tma_view(out) is not out:
             raise ValueError("attention: out must have q's shape, dtype and device, a contiguous last dimension, and strides and address in "
                              "multiples of 16 bytes")
-    lse = torch.full(q.shape[:-1], float("-inf"), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = torch.full(qs[:-1], float("-inf"), dtype=torch.float32, device=q.device) if return_lse else None
     if packed and B == 0:
-        if a.fill_rest:
+        if fill_rest:
             out.zero_()
     elif q.numel():
         q, k, v = _tma_view(q), _tma_view(k), _tma_view(v)
-        a.q_dev, a.k_dev, a.v_dev, a.out_dev = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-        a.lse_dev = lse.data_ptr() if return_lse else None
-        a.dtype, a.causal = _dt(q), 1 if causal else 0
-        a.batch, a.Tq, a.Tk, a.Hq, a.Hkv, a.D = B, Tq, Tk, Hq, Hkv, D
-        a.scale = scale
-        a.q_token_stride, a.q_head_stride = q.stride(-3), q.stride(-2)
-        a.k_token_stride, a.k_head_stride = k.stride(-3), k.stride(-2)
-        a.v_token_stride, a.v_head_stride = v.stride(-3), v.stride(-2)
-        a.out_token_stride, a.out_head_stride = out.stride(-3), out.stride(-2)
-        if not packed:
-            a.q_batch_stride, a.k_batch_stride, a.v_batch_stride, a.out_batch_stride = q.stride(0), k.stride(0), v.stride(0), out.stride(0)
-        lib = L.load()
-        need = L.check(lib.sq_attention_scratch_bytes(ctypes.byref(a)), "sq_attention_scratch_bytes")
-        scratch = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        first = 1 if packed else 0                     # packed tensors have no batch stride
+        strides = [(0, *t.stride()[:2]) if first else t.stride()[:3] for t in (q, k, v, out)]
+        a = L.AttentionArgs(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None,
+            _DT[dt], 1 if causal else 0, B, Tq, Tk, Hq, Hkv, D, 1 if fill_rest else 0,
+            *strides[0], *strides[1], *strides[2], *strides[3],
+            q_offsets.data_ptr() if packed else None, kv_offsets.data_ptr() if packed else None,
+            q_lens.data_ptr() if q_lens is not None else None, kv_lens.data_ptr() if kv_lens is not None else None,
+            scale, 0)
+        lib, ref = L.load(), ctypes.byref(a)
+        need = lib.sq_attention_scratch_bytes(ref)
+        if need < 0:
+            L.check(need, "sq_attention_scratch_bytes")
         if need:
+            scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
             a.scratch_dev, a.scratch_bytes = scratch.data_ptr(), need
-        with torch.cuda.device(q.device):
-            L.check(lib.sq_attention(ctypes.byref(a), _stream(q)), "sq_attention")
+        _run(lib.sq_attention, "sq_attention", q, ref)
         launch_count += 2 if need else 1
     return (out, lse) if return_lse else out
 
@@ -496,42 +511,25 @@ def gemm(kind, xq, wq, N, bounds, sx, sw, *, xq_neg=None, sx_neg=None, per_token
     batch = 1 if w_seg_as_batch else max(Bx, Bw)
     S = len(bounds) - 1
     w4 = kind == L.SQ_GEMM_W4A8
-    a = L.GemmArgs()
-    a.kind = kind
-    a.out_dtype = _DT[out_dtype]
-    a.batch, a.M, a.N, a.K = batch, M, N, K
-    a.xq_dev = xq.data_ptr()
-    a.xq_neg_dev = xq_neg.data_ptr() if xq_neg is not None else None
-    a.xq_batch_stride = M * K if (x_batched and Bx > 1) else 0
-    a.xq_row_stride = K
-    a.wq_dev = wq.data_ptr()
-    Kw = (bounds[1] - bounds[0]) if w_seg_as_batch else K
-    a.wq_row_stride = Kw // 2 if w4 else Kw
-    a.wq_batch_stride = N * a.wq_row_stride if Bw > 1 else 0
-    a.w_seg_as_batch = 1 if w_seg_as_batch else 0
-    a.num_segs = S
-    L.set_bounds(a.seg_bounds, bounds)
-    a.group_size = int(group_size or 0)
-    a.sw_is_bf16 = 1 if sw.dtype == torch.bfloat16 else 0
     if sw.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError("weight scales must be float32 or bfloat16")
-    a.sx_dev = sx.data_ptr()
-    a.sx_neg_dev = sx_neg.data_ptr() if sx_neg is not None else None
-    if per_token:
-        a.sx_batch_stride, a.sx_seg_stride, a.sx_row_stride = S * M, M, 1
-    else:
-        a.sx_batch_stride, a.sx_seg_stride, a.sx_row_stride = S, 1, 0
-    if sx_batch_stride is not None:
-        a.sx_batch_stride = sx_batch_stride
-    a.sw_dev = sw.data_ptr()
-    a.sw_batch_stride, a.sw_seg_stride, a.sw_group_stride, a.sw_col_stride = sw_strides
-    if bias is not None:
-        a.bias_dev = bias.data_ptr()
-        a.bias_dtype = _dt(bias)
-    a.bias_batch_stride = 0
+    if S > L.SQ_MAX_SEGS:
+        raise L.SegQuantError(L.SQ_ERR_INVALID_ARG, f"at most {L.SQ_MAX_SEGS} segments per call, got {S}")
+    Kw = (bounds[1] - bounds[0]) if w_seg_as_batch else K
+    w_row = Kw // 2 if w4 else Kw
+    sx_strides = (S * M, M, 1) if per_token else (S, 1, 0)
     y = out if out is not None else torch.empty((batch, M, N), dtype=out_dtype, device=xq.device)
-    a.y_dev = y.data_ptr()
-    a.y_batch_stride, a.y_row_stride = y_strides if y_strides is not None else (M * N, N)
+    y_bs, y_rs = y_strides if y_strides is not None else (M * N, N)
+    a = L.GemmArgs(
+        kind, _DT[out_dtype], batch, M, N, K,
+        xq.data_ptr(), xq_neg.data_ptr() if xq_neg is not None else None, M * K if (x_batched and Bx > 1) else 0, K,
+        wq.data_ptr(), N * w_row if Bw > 1 else 0, w_row, 1 if w_seg_as_batch else 0,
+        S, _Bounds(*bounds), int(group_size or 0), 1 if sw.dtype == torch.bfloat16 else 0,
+        sx.data_ptr(), sx_neg.data_ptr() if sx_neg is not None else None,
+        sx_strides[0] if sx_batch_stride is None else sx_batch_stride, sx_strides[1], sx_strides[2],
+        sw.data_ptr(), *sw_strides,
+        bias.data_ptr() if bias is not None else None, _dt(bias) if bias is not None else 0, 0, 0,
+        y.data_ptr(), y_bs, y_rs)
     if peer_outputs is not None:
         # fused all-gather: (device pointers of the peers' [M, *] buffers, row stride, column offset) in elements
         ptrs, prs, pco = peer_outputs
@@ -547,8 +545,7 @@ def gemm(kind, xq, wq, N, bounds, sx, sw, *, xq_neg=None, sx_neg=None, per_token
         sides = 2 if xq_neg is not None else 1
         acc = torch.zeros((batch, units, sides, M, N), dtype=torch.int32, device=xq.device)
         a.acc_dump_dev = acc.data_ptr()
-    with torch.cuda.device(xq.device):
-        L.check(L.load().sq_gemm(ctypes.byref(a), _stream(xq)), "sq_gemm")
+    _run(L.load().sq_gemm, "sq_gemm", xq, ctypes.byref(a))
     launch_count += 1
     return (y, acc) if want_acc else y
 
