@@ -8,6 +8,7 @@
 // thread keeps the sines of its columns in registers and walks the heads, which share them.  Everything else is fp32 with
 // one rounding at the end.
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -29,7 +30,7 @@ struct RotaryParams {
     int heads_per_cta;                // heads (of q, then of k) that one CTA's threads walk
     int group;                        // vector kernel: threads that share a row (power of two)
     int units;                        // vector kernel: threads of a group that have columns
-    float eps;
+    float eps, inv_d;                 // inv_d = 1 / D
     double turn[kRotMaxPairs];        // revolutions per unit of position
     unsigned char axis[kRotMaxPairs];
     short col[kRotMaxPairs];          // first column of a pair
@@ -48,137 +49,194 @@ __device__ __forceinline__ float2 rot_angle(const RotaryParams& p, long long b, 
     return make_float2(c, s);
 }
 
-// 8 elements <-> floats
+// A row's 8 columns as four pairs of floats, and back.
 template <typename T>
-__device__ __forceinline__ void rot_load8(const T* p, float (&v)[8]);
-template <>
-__device__ __forceinline__ void rot_load8<float>(const float* p, float (&v)[8]) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <>
-__device__ __forceinline__ void rot_load8<__half>(const __half* p, float (&v)[8]) {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void rot_unpack(const uint4& a, float2 (&v)[4]) {
     const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-    }
-}
-template <>
-__device__ __forceinline__ void rot_load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
-    const uint4 a = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        if constexpr (sizeof(T) == 4) v[i] = make_float2(0.0f, 0.0f);
+        else if constexpr (std::is_same<T, __half>::value) v[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        else v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
     }
 }
 template <typename T>
-__device__ __forceinline__ void rot_store8(T* p, const float (&v)[8]) {
-    if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const T lo = from_float<T>(v[2 * i]), hi = from_float<T>(v[2 * i + 1]);
-            w[i] = static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&lo)) | (static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(&hi)) << 16);
+struct RotRow {                       // 8 columns as loaded
+    uint4 w[sizeof(T) == 4 ? 2 : 1];
+    __device__ __forceinline__ void load(const T* p) {
+        w[0] = reinterpret_cast<const uint4*>(p)[0];       // plain loads: the result may overwrite the input
+        if constexpr (sizeof(T) == 4) w[1] = reinterpret_cast<const uint4*>(p)[1];
+    }
+    __device__ __forceinline__ void zero() {
+        w[0] = make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (sizeof(T) == 4) w[1] = w[0];
+    }
+    __device__ __forceinline__ void get(float2 (&v)[4]) const {
+        if constexpr (sizeof(T) == 4) {
+            v[0] = make_float2(__uint_as_float(w[0].x), __uint_as_float(w[0].y));
+            v[1] = make_float2(__uint_as_float(w[0].z), __uint_as_float(w[0].w));
+            v[2] = make_float2(__uint_as_float(w[1].x), __uint_as_float(w[1].y));
+            v[3] = make_float2(__uint_as_float(w[1].z), __uint_as_float(w[1].w));
+        } else {
+            rot_unpack<T>(w[0], v);
         }
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     }
-}
+    __device__ __forceinline__ void put(const float2 (&v)[4]) {
+        if constexpr (sizeof(T) == 4) {
+            w[0] = make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+            w[1] = make_uint4(__float_as_uint(v[2].x), __float_as_uint(v[2].y), __float_as_uint(v[3].x), __float_as_uint(v[3].y));
+        } else {
+            uint32_t o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (std::is_same<T, __half>::value) {
+                    const __half2 h = __float22half2_rn(v[i]);
+                    o[i] = *reinterpret_cast<const uint32_t*>(&h);
+                } else {
+                    const __nv_bfloat162 h = __float22bfloat162_rn(v[i]);
+                    o[i] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+            }
+            w[0] = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        reinterpret_cast<uint4*>(p)[0] = w[0];
+        if constexpr (sizeof(T) == 4) reinterpret_cast<uint4*>(p)[1] = w[1];
+    }
+};
 
 // A thread has one vector of 8 columns (adjacent pairs: 4 pairs) or two (halves: 8 pairs, one column of each in either
-// vector) of one token, and walks heads.  `group` threads share a row.
+// vector) of one token, and walks heads, the loads of kRotAhead heads in flight.  `group` threads share a row.  Two-wide fp32
+// instructions throughout: the kernel has about 50 instructions for 32 bytes of traffic and is near the issue limit with
+// scalar ones.
+constexpr int kRotAhead = 4;
+constexpr int kRotThreads = 128;
+constexpr int kRotWarps = 32;          // per SM; 48 to 96 measured the same or slower (64 x 64 grid, two samples: 23.8 against 24.4 to 26.0 us)
 template <typename T, bool HALVES, bool NORM>
-__global__ void __launch_bounds__(256) rotary_vec_kernel(const __grid_constant__ RotaryParams p) {
-    constexpr int NV = HALVES ? 2 : 1, NP = HALVES ? 8 : 4;
+__global__ void __launch_bounds__(kRotThreads) rotary_vec_kernel(const __grid_constant__ RotaryParams p) {
+    constexpr int NV = HALVES ? 2 : 1;
+    constexpr int U = (sizeof(T) == 4 || HALVES) ? kRotAhead / 2 : kRotAhead;
     const int u = threadIdx.x & (p.group - 1);
     const long long rows = p.batch * p.tokens;
     const long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) / p.group;
     const bool has = row < rows && u < p.units;
     const long long b = has ? row / p.tokens : 0, t = has ? row - b * p.tokens : 0;
-    int cols[NV];
-    float cs[NP], sn[NP];
     const int uu = has ? u : 0;
-    if constexpr (HALVES) {
-        cols[0] = p.unit_a[uu];
-        cols[1] = p.unit_b[uu];
-    } else {
-        cols[0] = 8 * uu;
-    }
+    const int col_a = HALVES ? p.unit_a[uu] : 8 * uu, col_b = HALVES ? p.unit_b[uu] : 0;
     const int pair0 = HALVES ? p.unit_pair[uu] : 4 * uu;
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-        float2 a = make_float2(1.0f, 0.0f);
-        if (has && pair0 >= 0 && pair0 + i < p.pairs) a = rot_angle(p, b, t, pair0 + i);
-        cs[i] = a.x;
-        sn[i] = a.y;
-    }
     const int h0 = blockIdx.y * p.heads_per_cta, h1 = min(h0 + p.heads_per_cta, p.heads[0] + p.heads[1]);
+    float2 cs[4 * NV], sn[4 * NV];    // adjacent: (c, c) and (-s, s) of a pair; halves: the pairs' cosines and sines two by two
+    bool angles = false;
 #pragma unroll
     for (int part = 0; part < 2; ++part) {
         const int first = part ? max(h0 - p.heads[0], 0) : h0, last = part ? h1 - p.heads[0] : min(h1, p.heads[0]);
         if (first >= last) continue;                                     // uniform over the CTA
-        const T* x = static_cast<const T*>(p.x[part]) + b * p.x_bs[part] + t * p.x_ts[part];
-        T* y = static_cast<T*>(p.y[part]) + b * p.y_bs[part] + t * p.y_ts[part];
-        float w[NV][8];
-        if constexpr (NORM) {
+        const T* x = static_cast<const T*>(p.x[part]) + b * p.x_bs[part] + t * p.x_ts[part] + first * p.x_hs[part];
+        T* y = static_cast<T*>(p.y[part]) + b * p.y_bs[part] + t * p.y_ts[part] + first * p.y_hs[part];
+        const long long xs = p.x_hs[part], ys = p.y_hs[part];
+        RotRow<T> in[U][NV];
+        auto fetch = [&](int h) {
 #pragma unroll
-            for (int v = 0; v < NV; ++v) rot_load8<T>(static_cast<const T*>(p.weight[part]) + cols[v], w[v]);
-        }
-#pragma unroll 4
-        for (int h = first; h < last; ++h) {
-            float e[NV][8];
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                if (has) {
-                    rot_load8<T>(x + h * p.x_hs[part] + cols[v], e[v]);
+            for (int i = 0; i < U; ++i) {
+                if (has && h + i < last) {
+                    in[i][0].load(x + i * xs + col_a);
+                    if constexpr (HALVES) in[i][NV - 1].load(x + i * xs + col_b);
                 } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) e[v][i] = 0.0f;
+                    in[i][0].zero();
+                    if constexpr (HALVES) in[i][NV - 1].zero();
                 }
             }
-            if constexpr (NORM) {
-                float ss = 0.0f;
-#pragma unroll
-                for (int v = 0; v < NV; ++v)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) ss = fmaf(e[v][i], e[v][i], ss);
-                for (int o = p.group >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                const float r = rsqrtf(ss / static_cast<float>(p.D) + p.eps);
-#pragma unroll
-                for (int v = 0; v < NV; ++v)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) e[v][i] *= r * w[v][i];
+            x += U * xs;
+        };
+        fetch(first);
+        float2 w[NV][4];
+        if constexpr (NORM) {
+            RotRow<T> r;
+            r.load(static_cast<const T*>(p.weight[part]) + col_a);
+            r.get(w[0]);
+            if constexpr (HALVES) {
+                r.load(static_cast<const T*>(p.weight[part]) + col_b);
+                r.get(w[NV - 1]);
             }
-            if (has) {
-                float o[NV][8];
+        }
+        if (!angles) {                                                   // while the first heads are on their way
+            angles = true;
 #pragma unroll
-                for (int i = 0; i < NP; ++i) {
+            for (int i = 0; i < 4 * NV; ++i) {
+                float2 a = make_float2(1.0f, 0.0f);
+                if (has && pair0 >= 0 && pair0 + i < p.pairs) a = rot_angle(p, b, t, pair0 + i);
+                if constexpr (HALVES) {
+                    if (i & 1) { cs[i >> 1].y = a.x; sn[i >> 1].y = a.y; }
+                    else { cs[i >> 1].x = a.x; sn[i >> 1].x = a.y; }
+                } else {
+                    cs[i] = make_float2(a.x, a.x);
+                    sn[i] = make_float2(-a.y, a.y);
+                }
+            }
+        }
+        for (int h = first; h < last; h += U) {
+            float2 e[U][NV][4];
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+#pragma unroll
+                for (int v = 0; v < NV; ++v) in[i][v].get(e[i][v]);
+            if (h + U < last) fetch(h + U);
+            if constexpr (NORM) {
+                float ss[U];
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    float2 s = __fmul2_rn(e[i][0][0], e[i][0][0]);
+#pragma unroll
+                    for (int v = 0; v < NV; ++v)
+#pragma unroll
+                        for (int k = v ? 0 : 1; k < 4; ++k) s = __ffma2_rn(e[i][v][k], e[i][v][k], s);
+                    ss[i] = s.x + s.y;
+                }
+                for (int o = p.group >> 1; o > 0; o >>= 1)
+#pragma unroll
+                    for (int i = 0; i < U; ++i) ss[i] += __shfl_xor_sync(0xffffffffu, ss[i], o);
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    const float r = rsqrtf(ss[i] * p.inv_d + p.eps);
+                    const float2 r2 = make_float2(r, r);
+#pragma unroll
+                    for (int v = 0; v < NV; ++v)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) e[i][v][k] = __fmul2_rn(e[i][v][k], __fmul2_rn(r2, w[v][k]));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                float2 o[NV][4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
                     if constexpr (HALVES) {
-                        o[0][i] = e[0][i] * cs[i] - e[1][i] * sn[i];
-                        o[1][i] = e[0][i] * sn[i] + e[1][i] * cs[i];
+                        const float2 m = make_float2(-sn[k].x, -sn[k].y);
+                        o[0][k] = __ffma2_rn(e[i][0][k], cs[k], __fmul2_rn(e[i][NV - 1][k], m));
+                        o[NV - 1][k] = __ffma2_rn(e[i][0][k], sn[k], __fmul2_rn(e[i][NV - 1][k], cs[k]));
                     } else {
-                        o[0][2 * i] = e[0][2 * i] * cs[i] - e[0][2 * i + 1] * sn[i];
-                        o[0][2 * i + 1] = e[0][2 * i] * sn[i] + e[0][2 * i + 1] * cs[i];
+                        o[0][k] = __ffma2_rn(e[i][0][k], cs[k], __fmul2_rn(make_float2(e[i][0][k].y, e[i][0][k].x), sn[k]));
                     }
                 }
-#pragma unroll
-                for (int v = 0; v < NV; ++v) rot_store8<T>(y + h * p.y_hs[part] + cols[v], o[v]);
+                if (has && h + i < last) {
+                    RotRow<T> r;
+                    r.put(o[0]);
+                    r.store(y + i * ys + col_a);
+                    if constexpr (HALVES) {
+                        r.put(o[NV - 1]);
+                        r.store(y + i * ys + col_b);
+                    }
+                }
             }
+            y += U * ys;
         }
     }
 }
 
 // Any width, stride and alignment: one warp per token, lane l has the pairs l, l + 32, ... and walks heads.
 template <typename T, bool NORM>
-__global__ void __launch_bounds__(256) rotary_scalar_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(kRotThreads) rotary_scalar_kernel(const __grid_constant__ RotaryParams p) {
     constexpr int NP = kRotMaxPairs / 32;
     const int lane = threadIdx.x & 31;
     const long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
@@ -207,7 +265,7 @@ __global__ void __launch_bounds__(256) rotary_scalar_kernel(const __grid_constan
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            r = rsqrtf(ss / static_cast<float>(p.D) + p.eps);
+            r = rsqrtf(ss * p.inv_d + p.eps);
         }
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
@@ -235,14 +293,14 @@ __global__ void __launch_bounds__(256) rotary_scalar_kernel(const __grid_constan
 template <typename T>
 static void launch_rotary(const RotaryParams& p, bool vec, bool halves, bool norm, dim3 grid, cudaStream_t st) {
     if (!vec) {
-        if (norm) rotary_scalar_kernel<T, true><<<grid, 256, 0, st>>>(p);
-        else rotary_scalar_kernel<T, false><<<grid, 256, 0, st>>>(p);
+        if (norm) rotary_scalar_kernel<T, true><<<grid, kRotThreads, 0, st>>>(p);
+        else rotary_scalar_kernel<T, false><<<grid, kRotThreads, 0, st>>>(p);
     } else if (halves) {
-        if (norm) rotary_vec_kernel<T, true, true><<<grid, 256, 0, st>>>(p);
-        else rotary_vec_kernel<T, true, false><<<grid, 256, 0, st>>>(p);
+        if (norm) rotary_vec_kernel<T, true, true><<<grid, kRotThreads, 0, st>>>(p);
+        else rotary_vec_kernel<T, true, false><<<grid, kRotThreads, 0, st>>>(p);
     } else {
-        if (norm) rotary_vec_kernel<T, false, true><<<grid, 256, 0, st>>>(p);
-        else rotary_vec_kernel<T, false, false><<<grid, 256, 0, st>>>(p);
+        if (norm) rotary_vec_kernel<T, false, true><<<grid, kRotThreads, 0, st>>>(p);
+        else rotary_vec_kernel<T, false, false><<<grid, kRotThreads, 0, st>>>(p);
     }
 }
 
@@ -316,18 +374,21 @@ int rotary(const sq_rotary_args* a, cudaStream_t st) {
     }
     p.pos = a->positions_dev; p.pos_float = a->positions_float ? 1 : 0;
     p.pos_bs = a->pos_batch_stride; p.pos_ts = a->pos_token_stride;
-    p.batch = a->batch; p.tokens = a->tokens; p.D = a->D; p.pairs = width / 2; p.eps = a->eps;
+    p.batch = a->batch; p.tokens = a->tokens; p.D = a->D; p.pairs = width / 2; p.eps = a->eps; p.inv_d = 1.0f / static_cast<float>(a->D);
     p.units = units;
     p.group = 1;
     while (p.group < units) p.group *= 2;
     const long long rows = a->batch * a->tokens;
     const long long threads = vec ? rows * p.group : rows * 32;
-    const long long ctas = (threads + 255) / 256;
-    // the heads of a token share its sines: cut them only as far as it takes to give every SM its threads
+    const long long ctas = (threads + kRotThreads - 1) / kRotThreads;
+    // The heads of a token share its sines: they are cut only as far as it takes to give every SM kRotWarps warps, into
+    // multiples of the heads that are loaded at a time.
     const int heads = a->heads_q + a->heads_k;
-    long long cuts = (8ll * kNumSMs + ctas - 1) / ctas;
+    const long long want = static_cast<long long>(kNumSMs) * kRotWarps * 32 / kRotThreads;
+    long long cuts = (want + ctas - 1) / ctas;
     if (cuts > heads) cuts = heads;
     p.heads_per_cta = static_cast<int>((heads + cuts - 1) / cuts);
+    if (p.heads_per_cta > kRotAhead) p.heads_per_cta = (p.heads_per_cta + kRotAhead - 1) / kRotAhead * kRotAhead;
     const dim3 grid(static_cast<unsigned>(ctas), static_cast<unsigned>((heads + p.heads_per_cta - 1) / p.heads_per_cta));
     SQ_REQUIRE(ctas < (1ll << 31), SQ_ERR_TOO_LARGE, "sq_rotary: too many rows");
     if (a->dtype == SQ_F32) launch_rotary<float>(p, vec, halves, norm, grid, st);

@@ -311,7 +311,7 @@ def rotary(q, k, positions, axes, *, theta=10000.0, pairing="adjacent", norm_q=N
                 raise ValueError("rotary: in place needs a contiguous last dimension")
             x = x.contiguous()
         if out is None:
-            out = torch.empty(x.shape, dtype=dt, device=x.device)
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
         elif out.shape != x.shape or out.dtype != dt or out.device != x.device or out.stride(-1) != 1:
             raise ValueError(f"rotary: out_{name} must have {name}'s shape, dtype and device and a contiguous last dimension")
         w = None if w is None else w.contiguous()
@@ -374,8 +374,10 @@ def attention(q, k, v, *, causal=False, scale=None, q_offsets=None, kv_offsets=N
     `out`, which has q's shape and dtype, D contiguous, strides and address multiples of 16 bytes, and overlaps no input.
     return_lse: also the float32 logarithm of the row sums, (B, Tq, Hq) or (Nq, Hq)."""
     global launch_count
-    _need_cuda(q, k, v)
-    _no_grad(q, k, v)
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        _need_cuda(q, k, v)
+    if q.requires_grad or k.requires_grad or v.requires_grad:
+        _no_grad(q, k, v)
     packed = q_offsets is not None
     if kv_offsets is not None and not packed:
         raise ValueError("attention: kv_offsets needs q_offsets")
@@ -412,7 +414,7 @@ def attention(q, k, v, *, causal=False, scale=None, q_offsets=None, kv_offsets=N
             kv_lens = _int32_list(kv_lens, B, "kv_lens", q.device)
     fill_rest = out is None
     if fill_rest:
-        out = torch.empty(qs, dtype=dt, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _need_cuda(out)
         if out.shape != qs or out.dtype != dt or out.device != q.device or _tma_view(out) is not out:
@@ -438,7 +440,7 @@ def attention(q, k, v, *, causal=False, scale=None, q_offsets=None, kv_offsets=N
         if need < 0:
             L.check(need, "sq_attention_scratch_bytes")
         if need:
-            scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+            scratch = q.new_empty(need, dtype=torch.uint8)
             a.scratch_dev, a.scratch_bytes = scratch.data_ptr(), need
         _run(lib.sq_attention, "sq_attention", q, ref)
         launch_count += 2 if need else 1
@@ -518,7 +520,7 @@ def gemm(kind, xq, wq, N, bounds, sx, sw, *, xq_neg=None, sx_neg=None, per_token
     Kw = (bounds[1] - bounds[0]) if w_seg_as_batch else K
     w_row = Kw // 2 if w4 else Kw
     sx_strides = (S * M, M, 1) if per_token else (S, 1, 0)
-    y = out if out is not None else torch.empty((batch, M, N), dtype=out_dtype, device=xq.device)
+    y = out if out is not None else xq.new_empty((batch, M, N), dtype=out_dtype)
     y_bs, y_rs = y_strides if y_strides is not None else (M * N, N)
     a = L.GemmArgs(
         kind, _DT[out_dtype], batch, M, N, K,
