@@ -24,6 +24,8 @@ namespace sq {
 
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();   // seg_gemm.cu
 long long wait_limit_cycles();                            // seg_gemm.cu
+// few rows against many keys (attention_rows.cu)
+int attention_rows(int dtype, const CUtensorMap& mk, const CUtensorMap& mv, const AttnParams& p, long long grid, cudaStream_t st);
 
 enum AttnWait : int { kAttnMma = 20, kAttnKvEmpty = 22, kAttnS = 23, kAttnPv = 26, kAttnTail = 27 };
 
@@ -584,6 +586,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const __grid_consta
     const int lane = threadIdx.x & 31;
     const long long r = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
     if (r >= p.rows) return;
+    cudaGridDependencySynchronize();
     const long long token = r / p.Hq;
     const int head = static_cast<int>(r - token * p.Hq);
     const int b = p.q_off ? 0 : static_cast<int>(token / p.Tq);
@@ -622,23 +625,43 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const __grid_consta
 // host side
 // ---------------------------------------------------------------------------------------------
 struct AttnPlan {
-    int P, tile_tokens, splits;
+    bool rows;                       // few rows against many keys: attention_rows.cu
+    int P, tile_tokens, splits, part_keys;
     long long tiles;                 // per chunk of heads
 };
 
+// The choice of kernel and of the parts goes by what the host knows: extents and heads, not the lengths on the device.
 static AttnPlan attention_plan(const sq_attention_args* a) {
     AttnPlan pl;
     const int G = a->Hq / a->Hkv;
+    const bool packed = a->q_offsets_dev != nullptr;
+    const long long avg = packed ? (a->Tq + a->batch - 1) / a->batch : a->Tq;      // query tokens of a sequence
+    pl.rows = avg * G <= 16;
+    const int most = pl.rows ? 16 : 32;
     pl.P = 1;
-    for (int d = 2; d <= G && d <= 32; ++d)
+    for (int d = 2; d <= G && d <= most; ++d)
         if (G % d == 0) pl.P = d;
-    pl.tile_tokens = 2 * (kAttnRows / pl.P);
-    pl.tiles = a->q_offsets_dev ? (a->Tq + a->batch * (pl.tile_tokens - 1)) / pl.tile_tokens + (a->fill_rest ? 2 : 0)
-                                : a->batch * ((a->Tq + pl.tile_tokens - 1) / pl.tile_tokens);
+    pl.tile_tokens = pl.rows ? 16 / pl.P : 2 * (kAttnRows / pl.P);
+    pl.tiles = packed ? (a->Tq + a->batch * (pl.tile_tokens - 1)) / pl.tile_tokens + (a->fill_rest ? 2 : 0)
+                      : a->batch * ((a->Tq + pl.tile_tokens - 1) / pl.tile_tokens);
     const long long items = pl.tiles * (a->Hq / pl.P);
-    const long long key_tiles = (a->Tk + kAttnKeys - 1) / kAttnKeys;
     pl.splits = 1;
-    if (items > 0 && items * 2 <= kNumSMs) {             // fewer CTAs than half the SMs: cut the keys into parts
+    pl.part_keys = 0;
+    if (items == 0 || a->Tk == 0) {
+        pl.part_keys = 1 << 30;
+        return pl;
+    }
+    if (pl.rows) {
+        // two CTAs to an SM and several rounds of them, so that sequences of different lengths even out; 128 keys a part at
+        // least, and at most as many parts as the joining warp has lanes
+        long long parts = (16ll * kNumSMs + items - 1) / items;
+        if (parts > 32) parts = 32;
+        long long keys = (a->Tk + parts - 1) / parts;
+        keys = (keys + 127) / 128 * 128;
+        pl.part_keys = static_cast<int>(keys);
+        pl.splits = static_cast<int>((a->Tk + keys - 1) / keys);
+    } else if (items * 2 <= kNumSMs) {                   // fewer CTAs than half the SMs: cut the keys into parts
+        const long long key_tiles = (a->Tk + kAttnKeys - 1) / kAttnKeys;
         long long s = kNumSMs / items;
         if (s > key_tiles / 2) s = key_tiles / 2;        // two key tiles a part at least
         if (s > 32) s = 32;
@@ -705,10 +728,23 @@ static int attention_launch(const CUtensorMap& mq, const CUtensorMap& mk, const 
     }
     attention_kernel<T, DP><<<static_cast<unsigned>(grid), kAttnThreads, C::kSmem, st>>>(mq, mk, mv, p);
     SQ_CUDA_OK(cudaGetLastError());
-    if (p.splits > 1) {
-        attention_join_kernel<T><<<static_cast<unsigned>((p.rows + 7) / 8), 256, 0, st>>>(p);
-        SQ_CUDA_OK(cudaGetLastError());
-    }
+    return SQ_OK;
+}
+
+// The joining kernel is launched while the one before it still runs (programmatic dependent launch) and waits inside for
+// its end: what is left of the second launch is the joining itself.
+template <typename T>
+static int attention_join(const AttnParams& p, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>((p.rows + 7) / 8));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    SQ_CUDA_OK(cudaLaunchKernelEx(&cfg, attention_join_kernel<T>, p));
     return SQ_OK;
 }
 
@@ -745,7 +781,9 @@ int attention(const sq_attention_args* a, cudaStream_t st) {
     p.fill_rest = a->fill_rest ? 1 : 0;
     p.causal = a->causal ? 1 : 0;
     p.Hq = a->Hq; p.Hkv = a->Hkv; p.D = a->D; p.G = a->Hq / a->Hkv; p.P = pl.P; p.chunks = static_cast<int>(chunks);
-    p.tile_tokens = pl.tile_tokens; p.tiles = static_cast<int>(pl.tiles); p.splits = pl.splits;
+    p.tile_tokens = pl.tile_tokens; p.tiles = static_cast<int>(pl.tiles); p.splits = pl.splits; p.part_keys = pl.part_keys;
+    p.q = a->q_dev;
+    p.q_bs = a->q_batch_stride; p.q_ts = a->q_token_stride; p.q_hs = a->q_head_stride;
     p.scale_log2 = a->scale * 1.4426950408889634f;
     p.o_bs = a->out_batch_stride; p.o_ts = a->out_token_stride; p.o_hs = a->out_head_stride;
     p.out = a->out_dev; p.lse = a->lse_dev;
@@ -758,19 +796,20 @@ int attention(const sq_attention_args* a, cudaStream_t st) {
 
     CUtensorMap mq, mk, mv;
     const uint64_t nb = packed ? 1 : a->batch;
-    {
+    if (!pl.rows || !keys) {
         const uint64_t dims[5] = {static_cast<uint64_t>(a->D), static_cast<uint64_t>(pl.P), static_cast<uint64_t>(chunks), static_cast<uint64_t>(a->Tq), nb};
         const uint64_t hs = a->q_head_stride * 2ull;
         const uint64_t sb[4] = {hs, hs * pl.P, a->q_token_stride * 2ull, a->q_batch_stride * 2ull};
-        const uint32_t box[5] = {64, static_cast<uint32_t>(pl.P), 1, static_cast<uint32_t>(pl.tile_tokens / 2), 1};
+        const uint32_t box[5] = {64, static_cast<uint32_t>(pl.P), 1, static_cast<uint32_t>(pl.tile_tokens / 2 > 0 ? pl.tile_tokens / 2 : 1), 1};
         rc = attention_map(&mq, a->q_dev, 5, dims, sb, box, "q");
         if (rc != SQ_OK) return rc;
     }
-    mk = mq;
-    mv = mq;
-    if (keys) {
+    if (!keys) {                                          // nothing is loaded; the kernels still take maps
+        mk = mq;
+        mv = mq;
+    } else {
         const uint64_t dims[4] = {static_cast<uint64_t>(a->D), static_cast<uint64_t>(a->Hkv), static_cast<uint64_t>(a->Tk), nb};
-        const uint32_t box[4] = {64, 1, kAttnKeys, 1};
+        const uint32_t box[4] = {64, 1, pl.rows ? 32u : static_cast<uint32_t>(kAttnKeys), 1};
         const uint64_t sk[3] = {a->k_head_stride * 2ull, a->k_token_stride * 2ull, a->k_batch_stride * 2ull};
         const uint64_t sv[3] = {a->v_head_stride * 2ull, a->v_token_stride * 2ull, a->v_batch_stride * 2ull};
         rc = attention_map(&mk, a->k_dev, 4, dims, sk, box, "k");
@@ -778,8 +817,15 @@ int attention(const sq_attention_args* a, cudaStream_t st) {
         rc = attention_map(&mv, a->v_dev, 4, dims, sv, box, "v");
         if (rc != SQ_OK) return rc;
     }
-    if (a->dtype == SQ_F16) return a->D <= 64 ? attention_launch<__half, 64>(mq, mk, mv, p, grid, st) : attention_launch<__half, 128>(mq, mk, mv, p, grid, st);
-    return a->D <= 64 ? attention_launch<__nv_bfloat16, 64>(mq, mk, mv, p, grid, st) : attention_launch<__nv_bfloat16, 128>(mq, mk, mv, p, grid, st);
+    if (pl.rows) {
+        rc = attention_rows(a->dtype, mk, mv, p, grid, st);
+    } else if (a->dtype == SQ_F16) {
+        rc = a->D <= 64 ? attention_launch<__half, 64>(mq, mk, mv, p, grid, st) : attention_launch<__half, 128>(mq, mk, mv, p, grid, st);
+    } else {
+        rc = a->D <= 64 ? attention_launch<__nv_bfloat16, 64>(mq, mk, mv, p, grid, st) : attention_launch<__nv_bfloat16, 128>(mq, mk, mv, p, grid, st);
+    }
+    if (rc != SQ_OK || p.splits == 1) return rc;
+    return a->dtype == SQ_F16 ? attention_join<__half>(p, st) : attention_join<__nv_bfloat16>(p, st);
 }
 
 long long attention_read_status() {

@@ -23,6 +23,7 @@ struct AttnParams {
     int tile_tokens;         // query tokens of a tile
     int tiles;               // upper bound on the number of tiles over all sequences
     int splits;              // parts that the keys of a tile are cut into
+    int part_keys;           // rows kernel: keys of a part (the large kernel cuts what a tile sees into equal parts)
     float scale_log2;        // scale * log2(e)
     long long q_bs, q_ts, q_hs, k_bs, k_ts, k_hs, v_bs, v_ts, v_hs, o_bs, o_ts, o_hs;   // element strides: batch, token, head
     const void* q;

@@ -23,6 +23,7 @@ static int g_last_tu = 0;   // (kind * 2 + dual) of the last launch; the trace r
 
 long long push_read_status();        // peer_push.cu
 long long attention_read_status();   // attention.cu
+long long attention_rows_read_status();
 
 long long read_device_status() {
     if (cudaDeviceSynchronize() != cudaSuccess) return SQ_ERR_CUDA;
@@ -40,8 +41,8 @@ long long read_device_status() {
         if (v < 0) return v;
         if (first == 0) first = v;
     }
-    {
-        const long long v = attention_read_status();
+    for (const auto read : {attention_read_status, attention_rows_read_status}) {
+        const long long v = read();
         if (v < 0) return v;
         if (first == 0) first = v;
     }
