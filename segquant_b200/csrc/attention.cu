@@ -32,7 +32,7 @@ enum AttnWait : int { kAttnMma = 20, kAttnKvEmpty = 22, kAttnS = 23, kAttnPv = 2
 constexpr int kAttnThreads = 384;
 // Of kPolyOf pairs of exponentials, kPoly go to the FMA pipe (ex2_poly).  The special-function pipe does 4 lanes a cycle: two
 // warps' 128 exponentials a row take 2048 cycles there while everything else that a tile needs takes about 1000.
-constexpr int kPoly = 1, kPolyOf = 4;
+constexpr int kPoly = 1, kPolyOf = 6;
 constexpr int kWarpMma = 9;         // and the next one
 constexpr int kAttnRows = 128;       // rows of a sub-tile = tensor-memory lanes
 constexpr int kAttnKeys = 128;       // keys of a tile
@@ -534,30 +534,30 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             T* out = static_cast<T*>(p.out) + static_cast<long long>(T0.b) * p.o_bs + static_cast<long long>(T0.q_base + tok) * p.o_ts +
                      static_cast<long long>(head) * p.o_hs;
             float* part = p.part_o + (split * p.rows + r) * p.D;
-            for (int i = 0; i < p.D; i += 16) {               // whole warps: tcgen05.ld
-                uint32_t o[16];
-                if (nt > 0) {
-                    tmem_ld_x16(to + i, o);
-                    tmem_ld_wait_x16(o);
-                } else {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = 0u;
+            for (int i0 = 0; i0 < DP; i0 += 64) {             // whole warps: tcgen05.ld; 64 columns a round trip
+                uint32_t o[64];
+                if (nt > 0) {
+                    tmem_ld_x32(to + i0, o);
+                    tmem_ld_x32(to + i0 + 32, o + 32);
+                    tmem_ld_wait_x32(o);
+                    tmem_ld_wait_x32(o + 32);
                 }
                 if (!mine) continue;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = empty ? 0u : __float_as_uint(__uint_as_float(o[e]) * inv);
+                for (int i = 0; i < 64; ++i) o[i] = empty ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
                 if (p.splits > 1) {
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        if (i + e < p.D && nt > 0) *reinterpret_cast<uint4*>(part + i + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    for (int i = 0; i < 64; i += 4)
+                        if (i0 + i < p.D && !empty) *reinterpret_cast<uint4*>(part + i0 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < 16; e += 8) {
-                        if (i + e < p.D) {
+                    for (int i = 0; i < 64; i += 8) {
+                        if (i0 + i < p.D) {
                             uint32_t w[4];
 #pragma unroll
-                            for (int x = 0; x < 4; ++x) w[x] = pack2<T>(__uint_as_float(o[e + 2 * x]), __uint_as_float(o[e + 2 * x + 1]));
-                            *reinterpret_cast<uint4*>(out + i + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                            for (int x = 0; x < 4; ++x) w[x] = pack2<T>(__uint_as_float(o[i + 2 * x]), __uint_as_float(o[i + 2 * x + 1]));
+                            *reinterpret_cast<uint4*>(out + i0 + i) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
                     }
                 }
