@@ -642,9 +642,9 @@ static AttnPlan attention_plan(const sq_attention_args* a) {
     for (int d = 2; d <= G && d <= most; ++d)
         if (G % d == 0) pl.P = d;
     pl.tile_tokens = pl.rows ? 16 / pl.P : 2 * (kAttnRows / pl.P);
-    pl.tiles = packed ? (a->Tq + a->batch * (pl.tile_tokens - 1)) / pl.tile_tokens + (a->fill_rest ? 2 : 0)
-                      : a->batch * ((a->Tq + pl.tile_tokens - 1) / pl.tile_tokens);
-    const long long items = pl.tiles * (a->Hq / pl.P);
+    pl.tiles = packed ? (a->Tq + a->batch * (pl.tile_tokens - 1)) / pl.tile_tokens : a->batch * ((a->Tq + pl.tile_tokens - 1) / pl.tile_tokens);
+    const long long items = pl.tiles * (a->Hq / pl.P);   // the parts do not depend on fill_rest: the result's bits do not either
+    if (packed && a->fill_rest) pl.tiles += 2;
     pl.splits = 1;
     pl.part_keys = 0;
     if (items == 0 || a->Tk == 0) {

@@ -26,7 +26,7 @@ struct RotaryParams {
     long long pos_bs, pos_ts;
     long long batch, tokens;          // tokens of one batch entry
     int D, pairs;                     // rotated pairs
-    int pos_float;
+    int pos_float, halves;
     int heads_per_cta;                // heads (of q, then of k) that one CTA's threads walk
     int group;                        // vector kernel: threads that share a row (power of two)
     int units;                        // vector kernel: threads of a group that have columns
@@ -242,6 +242,7 @@ __global__ void __launch_bounds__(kRotThreads) rotary_scalar_kernel(const __grid
     const long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
     if (row >= p.batch * p.tokens) return;
     const long long b = row / p.tokens, t = row - b * p.tokens;
+    const bool halves = p.halves != 0;
     float cs[NP], sn[NP];
 #pragma unroll
     for (int i = 0; i < NP; ++i)
@@ -277,8 +278,9 @@ __global__ void __launch_bounds__(kRotThreads) rotary_scalar_kernel(const __grid
                     u *= r * to_float<T>(w[a]);
                     v *= r * to_float<T>(w[c]);
                 }
-                y[a] = from_float<T>(u * cs[i] - v * sn[i]);
-                y[c] = from_float<T>(u * sn[i] + v * cs[i]);
+                // the vector kernel's products and sums, so that a layout does not show in the result
+                y[a] = from_float<T>(fmaf(u, cs[i], __fmul_rn(v, -sn[i])));
+                y[c] = from_float<T>(halves ? fmaf(u, sn[i], __fmul_rn(v, cs[i])) : fmaf(v, cs[i], __fmul_rn(u, sn[i])));
             }
         }
         for (int i = 2 * p.pairs + lane; i < p.D; i += 32) {
@@ -372,7 +374,7 @@ int rotary(const sq_rotary_args* a, cudaStream_t st) {
         const long long n[6] = {a->batch, a->tokens, t.heads, a->batch, a->tokens, t.heads};
         for (int j = 0; j < 6; ++j) vec = vec && (n[j] == 1 || t.s[j] * es % 16 == 0);
     }
-    p.pos = a->positions_dev; p.pos_float = a->positions_float ? 1 : 0;
+    p.pos = a->positions_dev; p.pos_float = a->positions_float ? 1 : 0; p.halves = halves ? 1 : 0;
     p.pos_bs = a->pos_batch_stride; p.pos_ts = a->pos_token_stride;
     p.batch = a->batch; p.tokens = a->tokens; p.D = a->D; p.pairs = width / 2; p.eps = a->eps; p.inv_d = 1.0f / static_cast<float>(a->D);
     p.units = units;
