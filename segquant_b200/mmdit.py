@@ -14,7 +14,9 @@ would give it (segquant/pattern_detector.py:239-358):
   * attention output projections: S = 1 by default, or 24 K-segments of 64 (`out_proj_segments=24`,
     the reshape_to_linear pattern: heads x head_dim);
   * everything else: S = 1.
-Attention (torch SDPA) stays bf16.  Scales are calibrated once from one forward of the float model on the
+Attention (torch SDPA, or with attention="fused" this library's kernel) stays bf16; `rotary_axes` and `qk_norm` put rotary positions
+and the RMS normalisation of the heads in front of it (one kernel, in place in the joint q | k | v buffer), and
+`modulation_weights="int4"` stores the adaLN projections in 4 bits.  Scales are calibrated once from one forward of the float model on the
 given inputs (AMax), then every layer runs the fused quantise + tcgen05 GEMM path; where a LayerNorm + adaLN
 modulation feeds linears, one kernel normalises, modulates and quantises (FusedNorm below), q / k / v of a stream
 run as one GEMM on those bytes, the GELU in front of the MLP down-projection is evaluated inside its quantise kernel,
@@ -228,12 +230,34 @@ class _InLine:
         return contextlib.nullcontext()
 
 
+def grid_positions(img_tokens, txt_tokens, device):
+    """int32 (img_tokens + txt_tokens, 3) positions (sequence, row, column) in the order of a block's joint buffer: image tokens
+    on a square grid at sequence position 0, text tokens behind them along the sequence axis alone."""
+    side = math.isqrt(img_tokens)
+    if side * side != img_tokens:
+        raise ValueError(f"{img_tokens} image tokens are not a square grid")
+    i = torch.arange(img_tokens, device=device)
+    img = torch.stack([torch.zeros_like(i), i // side, i % side], dim=1)
+    j = torch.arange(1, txt_tokens + 1, device=device)
+    return torch.cat([img, torch.stack([j, torch.zeros_like(j), torch.zeros_like(j)], dim=1)]).to(torch.int32)
+
+
 class JointBlock:
-    def __init__(self, hidden, heads, gen, device, dtype, last, out_proj_segments):
+    def __init__(self, hidden, heads, gen, device, dtype, last, out_proj_segments, attention="torch", rotary_axes=None, qk_norm=False,
+                 modulation_weights="int8"):
+        """attention: "torch" (scaled_dot_product_attention) or "fused" (ops.attention); rotary_axes: widths of the heads' blocks for
+        the axes of `positions` (set by the caller, see grid_positions); qk_norm: RMS normalisation of the heads of q and k."""
+        if attention not in ("torch", "fused"):
+            raise ValueError('attention must be "torch" or "fused"')
+        if qk_norm and rotary_axes is None:
+            raise ValueError("qk_norm rides on the rotary kernel: give rotary_axes")
+        self.attention, self.rotary_axes, self.positions = attention, rotary_axes, None
+        ones = torch.ones(hidden // heads, dtype=dtype, device=device) if qk_norm else None
+        self.norm_q, self.norm_k = ones, ones
         self.heads, self.last = heads, last
         mk = lambda i, o, **kw: QLinear(i, o, gen, device, dtype, **kw)  # noqa: E731
-        self.norm1 = mk(hidden, 6 * hidden, chunks=6, dual=True)
-        self.norm1_context = mk(hidden, (2 if last else 6) * hidden, chunks=2 if last else 6, dual=True)
+        self.norm1 = mk(hidden, 6 * hidden, chunks=6, dual=True, wq=modulation_weights)
+        self.norm1_context = mk(hidden, (2 if last else 6) * hidden, chunks=2 if last else 6, dual=True, wq=modulation_weights)
         self.to_q, self.to_k, self.to_v = mk(hidden, hidden), mk(hidden, hidden), mk(hidden, hidden)
         self.add_q, self.add_k, self.add_v = mk(hidden, hidden), mk(hidden, hidden), mk(hidden, hidden)
         seg = dict(seg_mode="input", chunks=out_proj_segments) if out_proj_segments > 1 else {}
@@ -272,11 +296,18 @@ class JointBlock:
         _, img = norm_call((self.to_q, self.to_k, self.to_v), img, m[0], m[1], [qkv[:, :Ti, j] for j in range(3)], pend_img)
         side.join()
 
-        def heads(t):
-            return t.view(B, Ti + Tt, self.heads, H // self.heads).transpose(1, 2)
-
-        a = F.scaled_dot_product_attention(heads(qkv[:, :, 0]), heads(qkv[:, :, 1]), heads(qkv[:, :, 2]))
-        a = a.transpose(1, 2).reshape(B, Ti + Tt, H)
+        q, k, v = (qkv[:, :, j].view(B, Ti + Tt, self.heads, H // self.heads) for j in range(3))
+        if self.rotary_axes is not None:
+            from . import ops
+            if self.positions is None:
+                raise RuntimeError("rotary_axes needs the block's positions")
+            ops.rotary(q, k, self.positions, self.rotary_axes, norm_q=self.norm_q, norm_k=self.norm_k, out_q=q, out_k=k)
+        if self.attention == "fused":
+            from . import ops
+            a = ops.attention(q, k, v).view(B, Ti + Tt, H)
+        else:
+            a = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
+            a = a.transpose(1, 2).reshape(B, Ti + Tt, H)
         a_img, a_txt = a[:, :Ti], a[:, Ti:]
         side.fork()
 
@@ -320,7 +351,7 @@ def quantized_calls(fused_norm=None):
 
 class SyntheticMMDiT:
     def __init__(self, device, blocks=24, hidden=1536, heads=24, img_tokens=4096, txt_tokens=333, seed=0,
-                 dtype=torch.bfloat16, out_proj_segments=1):
+                 dtype=torch.bfloat16, out_proj_segments=1, attention="torch", rotary_axes=None, qk_norm=False, modulation_weights="int8"):
         gen = torch.Generator().manual_seed(seed)
         self.device, self.dtype, self.hidden = device, dtype, hidden
         self.img_tokens, self.txt_tokens = img_tokens, txt_tokens
@@ -328,8 +359,13 @@ class SyntheticMMDiT:
         self.context_embedder = mk(4096, hidden)
         self.t_lin1, self.t_lin2 = mk(256, hidden), mk(hidden, hidden, dual=True)
         self.p_lin1, self.p_lin2 = mk(2048, hidden), mk(hidden, hidden, dual=True)
-        self.blocks = [JointBlock(hidden, heads, gen, device, dtype, last=(i == blocks - 1), out_proj_segments=out_proj_segments)
+        self.blocks = [JointBlock(hidden, heads, gen, device, dtype, last=(i == blocks - 1), out_proj_segments=out_proj_segments, attention=attention,
+                                  rotary_axes=rotary_axes, qk_norm=qk_norm, modulation_weights=modulation_weights)
                        for i in range(blocks)]
+        if rotary_axes is not None:
+            positions = grid_positions(img_tokens, txt_tokens, device)
+            for b in self.blocks:
+                b.positions = positions
         self.norm_out = mk(hidden, 2 * hidden, chunks=2, dual=True)
         self.proj_out = mk(hidden, 64)
         self.calibrated = False
