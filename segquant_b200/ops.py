@@ -9,6 +9,7 @@ The two functions at the bottom keep the tensor contract of the reference's pybi
 layer forward that SegmentLinear uses.
 """
 import ctypes
+import struct
 
 import torch
 
@@ -24,8 +25,6 @@ KERNELS = {
     "Wint4Aint8": (L.SQ_GEMM_W4A8, L.SQ_Q_INT8, L.SQ_Q_INT4),
 }
 
-_Bounds = ctypes.c_int32 * (L.SQ_MAX_SEGS + 1)
-
 launch_count = 0  # kernels of this library launched by this process (bench.py reports it)
 
 
@@ -33,15 +32,24 @@ def _stream(t):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
-def _run(fn, what, t, *args):
-    """Calls a C entry point with the current stream of t's device (made current for the call if it is not) and checks its status.
-    Spelled out without context managers where it can be: a small operator is done before its Python call returns."""
-    dev = t.get_device()
+# Argument blocks of the operators that are short enough for their Python call to count, packed in one go (setting the fields of
+# a ctypes.Structure one by one takes three times as long); the layouts are those of _lib's structures.
+_GEMM = struct.Struct("@ii4qPPqqPqqii%dsiiPPqqqPqqqqPiiqPqqPii%dPqq" % (4 * (L.SQ_MAX_SEGS + 1), L.SQ_MAX_PEERS))
+_ATTENTION = struct.Struct("@5Pii3qiiii12q4PfiPq")
+_ROTARY = struct.Struct("@4Piiqqiiii%ds12qPqqifdPP" % (4 * L.SQ_ROTARY_MAX_AXES))
+assert (_GEMM.size, _ATTENTION.size, _ROTARY.size) == tuple(ctypes.sizeof(c) for c in (L.GemmArgs, L.AttentionArgs, L.RotaryArgs))
+_NO_PEERS = (0,) * L.SQ_MAX_PEERS
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _run(fn, what, dev, *args):
+    """Calls a C entry point with the current stream of device `dev` (made current for the call if it is not) and checks its
+    status.  Without a context manager where it can be: a small operator is done before its Python call returns."""
     if torch.cuda.current_device() == dev:
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+        status = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+            status = fn(*args, _raw_stream(dev))
     if status < 0:
         L.check(status, what)
 
@@ -254,7 +262,6 @@ def quantize_act_dynamic(x, bounds, out_kind=L.SQ_Q_INT8, dual=False, smooth=Non
 # ---------------------------------------------------------------------------------------------
 # rotary positions
 # ---------------------------------------------------------------------------------------------
-_Axes = ctypes.c_int32 * L.SQ_ROTARY_MAX_AXES
 PAIRINGS = {"adjacent": L.SQ_ROTARY_ADJACENT, "halves": L.SQ_ROTARY_HALVES}
 
 
@@ -268,71 +275,71 @@ def rotary(q, k, positions, axes, *, theta=10000.0, pairing="adjacent", norm_q=N
     float32, float16 and bfloat16, D up to 256; arithmetic in fp32 (angles in fp64), rounded once.  out_q / out_k may be q / k
     themselves.  Returns (q, k) rotated; (q, None) without k."""
     global launch_count
-    _need_cuda(q, k, positions, norm_q, norm_k, out_q, out_k)
-    _no_grad(q, k, norm_q, norm_k)
+    dev = q.get_device()
+    if not q.is_cuda or not positions.is_cuda or not (k is None or k.is_cuda):
+        _need_cuda(q, k, positions)
+    if q.requires_grad or (k is not None and k.requires_grad) or (norm_q is not None and norm_q.requires_grad) or (norm_k is not None and norm_k.requires_grad):
+        _no_grad(q, k, norm_q, norm_k)
     if pairing not in PAIRINGS:
         raise ValueError(f"pairing must be one of {list(PAIRINGS)}")
-    qs, dt = q.shape, q.dtype
+    qs, dt, A = q.shape, q.dtype, len(axes)
     if len(qs) not in (3, 4) or (k is not None and (k.shape[:-2] != qs[:-2] or k.shape[-1] != qs[-1])):
         raise ValueError("rotary: q (B, T, Hq, D) and k (B, T, Hk, D), or packed (N, H, D) ones")
-    if k is not None and (k.dtype != dt or k.device != q.device):
+    if k is not None and (k.dtype != dt or k.get_device() != dev):
         raise TypeError("rotary: q and k must share dtype and device")
-    if len(axes) == 0 or len(axes) > L.SQ_ROTARY_MAX_AXES:
+    if A == 0 or A > L.SQ_ROTARY_MAX_AXES:
         raise ValueError(f"rotary: 1 to {L.SQ_ROTARY_MAX_AXES} axes")
     B, T = (1, qs[0]) if len(qs) == 3 else qs[:2]
     D = qs[-1]
-    if positions.shape[-2:] != (T, len(axes)) or (positions.dim() != 2 and tuple(positions.shape) != (B, T, len(axes))):
-        raise ValueError(f"rotary: positions must be {(T, len(axes))} or {(B, T, len(axes))}, not {tuple(positions.shape)}")
-    if positions.dtype not in (torch.int32, torch.float32) or positions.device != q.device:
+    ps = positions.shape
+    if ps != (T, A) and ps != (B, T, A):
+        raise ValueError(f"rotary: positions must be {(T, A)} or {(B, T, A)}, not {tuple(ps)}")
+    if positions.dtype not in (torch.int32, torch.float32) or positions.get_device() != dev:
         raise TypeError("rotary: positions must be int32 or float32 on q's device")
-    if k is not None and (norm_q is None) != (norm_k is None):
-        raise ValueError("rotary: norm_q and norm_k come together")
-    if k is None and norm_k is not None:
-        raise ValueError("rotary: norm_k without k")
-    for w in (norm_q, norm_k):
-        if w is not None and (w.shape != (D,) or w.dtype != dt or w.device != q.device):
-            raise ValueError("rotary: norm weights must be (D,) tensors of q's dtype on its device")
+    if (norm_k is not None and k is None) or (k is not None and (norm_q is None) != (norm_k is None)):
+        raise ValueError("rotary: norm_q and norm_k come together, norm_k with k")
     positions = positions.contiguous()
-    keep, outs, ptrs, out_ptrs, heads, strides, out_strides, norms = [], [], [], [], [], [], [], []
-    for name, x, out, w in (("q", q, out_q, norm_q), ("k", k, out_k, norm_k)):
-        if x is None:
-            if out is not None:
-                raise ValueError(f"rotary: out_{name} without {name}")
-            outs.append(None)
-            ptrs.append(None)
-            out_ptrs.append(None)
-            norms.append(None)
-            heads.append(0)
-            strides += (0, 0, 0)
-            out_strides += (0, 0, 0)
-            continue
-        if x.stride(-1) != 1:
-            if out is x:
-                raise ValueError("rotary: in place needs a contiguous last dimension")
-            x = x.contiguous()
-        if out is None:
-            out = torch.empty_like(x, memory_format=torch.contiguous_format)
-        elif out.shape != x.shape or out.dtype != dt or out.device != x.device or out.stride(-1) != 1:
-            raise ValueError(f"rotary: out_{name} must have {name}'s shape, dtype and device and a contiguous last dimension")
-        w = None if w is None else w.contiguous()
-        keep += (x, w)
-        outs.append(out)
-        ptrs.append(x.data_ptr())
-        out_ptrs.append(out.data_ptr())
-        norms.append(None if w is None else w.data_ptr())
-        heads.append(x.shape[-2])
-        for t, into in ((x, strides), (out, out_strides)):
-            st = t.stride()
-            into += st[:3] if len(st) == 4 else (0, *st[:2])
-    A = len(axes)
-    a = L.RotaryArgs(
-        ptrs[0], ptrs[1], out_ptrs[0], out_ptrs[1], _dt(q), PAIRINGS[pairing], B, T, heads[0], heads[1], D, A, _Axes(*axes),
-        *strides, *out_strides, positions.data_ptr(), T * A if positions.dim() == 3 else 0, A,
-        1 if positions.dtype == torch.float32 else 0, eps, theta, norms[0], norms[1])
-    _run(L.load().sq_rotary, "sq_rotary", q, ctypes.byref(a))
-    if B * T * (heads[0] + heads[1]):
+    nq = nk = 0
+    if norm_q is not None:
+        for w in (norm_q, norm_k):
+            if w is not None and (w.shape != (D,) or w.dtype != dt or w.get_device() != dev):
+                raise ValueError("rotary: norm weights must be (D,) tensors of q's dtype on its device")
+        norm_q = norm_q.contiguous()
+        nq = norm_q.data_ptr()
+        if norm_k is not None:
+            norm_k = norm_k.contiguous()
+            nk = norm_k.data_ptr()
+    q, out_q, qi, qo = _rotary_pair(q, out_q, "q")
+    if k is not None:
+        k, out_k, ki, ko = _rotary_pair(k, out_k, "k")
+        a = (q.data_ptr(), k.data_ptr(), out_q.data_ptr(), out_k.data_ptr(), _dt(q), PAIRINGS[pairing], B, T, qs[-2], k.shape[-2])
+    elif out_k is not None:
+        raise ValueError("rotary: out_k without k")
+    else:
+        ki = ko = (0, 0, 0)
+        a = (q.data_ptr(), 0, out_q.data_ptr(), 0, _dt(q), PAIRINGS[pairing], B, T, qs[-2], 0)
+    a = _ROTARY.pack(*a, D, A, struct.pack(f"{A}i", *axes), *qi, *ki, *qo, *ko, positions.data_ptr(), T * A if len(ps) == 3 else 0, A,
+                     1 if positions.dtype == torch.float32 else 0, eps, theta, nq, nk)
+    _run(L.load().sq_rotary, "sq_rotary", dev, a)
+    if q.numel():
         launch_count += 1
-    return tuple(outs)
+    return out_q, out_k
+
+
+def _rotary_pair(x, out, name):
+    """(input, output, their (batch, token, head) strides)"""
+    xs = x.stride()
+    if xs[-1] != 1 and x.numel():
+        if out is x:
+            raise ValueError("rotary: in place needs a contiguous last dimension")
+        x = x.contiguous()
+        xs = x.stride()
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    elif out is not x and (out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1):
+        raise ValueError(f"rotary: out_{name} must have {name}'s shape, dtype and device and a contiguous last dimension")
+    os = out.stride()
+    return (x, out, xs[:3], os[:3]) if len(xs) == 4 else (x, out, (0, xs[0], xs[1]), (0, os[0], os[1]))
 
 
 # ---------------------------------------------------------------------------------------------
@@ -353,9 +360,9 @@ def _tma_view(t):
     return t.clone(memory_format=torch.contiguous_format)
 
 
-def _int32_list(t, n, name, device):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or t.device != device:
-        raise ValueError(f"attention: {name} must be an int32 tensor of {n} elements on {device}")
+def _int32_list(t, n, name, dev):
+    if t.dtype != torch.int32 or t.shape != (n,) or t.get_device() != dev or not t.is_cuda:
+        raise ValueError(f"attention: {name} must be an int32 tensor of {n} elements on cuda:{dev}")
     return t.contiguous()
 
 
@@ -389,7 +396,8 @@ def attention(q, k, v, *, causal=False, scale=None, q_offsets=None, kv_offsets=N
     rank = 3 if packed else 4
     if len(qs) != rank or len(ks) != rank or v.shape != ks or ks[-1] != qs[-1] or (not packed and ks[0] != qs[0]):
         raise ValueError("attention: q (B, Tq, Hq, D) with k, v (B, Tk, Hkv, D), or packed q (Nq, Hq, D) with k, v (Nk, Hkv, D)")
-    if k.device != q.device or v.device != q.device:
+    dev = q.get_device()
+    if k.get_device() != dev or v.get_device() != dev:
         raise ValueError("attention: q, k and v must be on one device")
     Tq, Hq, D = qs[-3:]
     Tk, Hkv = ks[-3:-1]
@@ -405,13 +413,13 @@ def attention(q, k, v, *, causal=False, scale=None, q_offsets=None, kv_offsets=N
         B = q_offsets.numel() - 1
         if B < 0:
             raise ValueError("attention: q_offsets needs at least one element")
-        q_offsets, kv_offsets = _int32_list(q_offsets, B + 1, "q_offsets", q.device), _int32_list(kv_offsets, B + 1, "kv_offsets", q.device)
+        q_offsets, kv_offsets = _int32_list(q_offsets, B + 1, "q_offsets", dev), _int32_list(kv_offsets, B + 1, "kv_offsets", dev)
     else:
         B = qs[0]
         if q_lens is not None:
-            q_lens = _int32_list(q_lens, B, "q_lens", q.device)
+            q_lens = _int32_list(q_lens, B, "q_lens", dev)
         if kv_lens is not None:
-            kv_lens = _int32_list(kv_lens, B, "kv_lens", q.device)
+            kv_lens = _int32_list(kv_lens, B, "kv_lens", dev)
     fill_rest = out is None
     if fill_rest:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -425,24 +433,26 @@ def attention(q, k, v, *, causal=False, scale=None, q_offsets=None, kv_offsets=N
         if fill_rest:
             out.zero_()
     elif q.numel():
-        q, k, v = _tma_view(q), _tma_view(k), _tma_view(v)
-        first = 1 if packed else 0                     # packed tensors have no batch stride
-        strides = [(0, *t.stride()[:2]) if first else t.stride()[:3] for t in (q, k, v, out)]
-        a = L.AttentionArgs(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else None,
-            _DT[dt], 1 if causal else 0, B, Tq, Tk, Hq, Hkv, D, 1 if fill_rest else 0,
-            *strides[0], *strides[1], *strides[2], *strides[3],
-            q_offsets.data_ptr() if packed else None, kv_offsets.data_ptr() if packed else None,
-            q_lens.data_ptr() if q_lens is not None else None, kv_lens.data_ptr() if kv_lens is not None else None,
-            scale, 0)
-        lib, ref = L.load(), ctypes.byref(a)
-        need = lib.sq_attention_scratch_bytes(ref)
+        qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        if (qp | kp | vp) & 15 or not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous()):
+            q, k, v = _tma_view(q), _tma_view(k), _tma_view(v)
+            qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        sq, sk, sv, so = q.stride(), k.stride(), v.stride(), out.stride()
+        if packed:                                     # no batch stride
+            strides = (0, sq[0], sq[1], 0, sk[0], sk[1], 0, sv[0], sv[1], 0, so[0], so[1])
+        else:
+            strides = (*sq[:3], *sk[:3], *sv[:3], *so[:3])
+        head = (qp, kp, vp, out.data_ptr(), lse.data_ptr() if return_lse else 0, _DT[dt], 1 if causal else 0, B, Tq, Tk, Hq, Hkv, D, 1 if fill_rest else 0,
+                *strides, q_offsets.data_ptr() if packed else 0, kv_offsets.data_ptr() if packed else 0,
+                q_lens.data_ptr() if q_lens is not None else 0, kv_lens.data_ptr() if kv_lens is not None else 0, scale, 0)
+        lib, a = L.load(), _ATTENTION.pack(*head, 0, 0)
+        need = lib.sq_attention_scratch_bytes(a)
         if need < 0:
             L.check(need, "sq_attention_scratch_bytes")
         if need:
             scratch = q.new_empty(need, dtype=torch.uint8)
-            a.scratch_dev, a.scratch_bytes = scratch.data_ptr(), need
-        _run(lib.sq_attention, "sq_attention", q, ref)
+            a = _ATTENTION.pack(*head, scratch.data_ptr(), need)
+        _run(lib.sq_attention, "sq_attention", dev, a)
         launch_count += 2 if need else 1
     return (out, lse) if return_lse else out
 
@@ -522,32 +532,29 @@ def gemm(kind, xq, wq, N, bounds, sx, sw, *, xq_neg=None, sx_neg=None, per_token
     sx_strides = (S * M, M, 1) if per_token else (S, 1, 0)
     y = out if out is not None else xq.new_empty((batch, M, N), dtype=out_dtype)
     y_bs, y_rs = y_strides if y_strides is not None else (M * N, N)
-    a = L.GemmArgs(
-        kind, _DT[out_dtype], batch, M, N, K,
-        xq.data_ptr(), xq_neg.data_ptr() if xq_neg is not None else None, M * K if (x_batched and Bx > 1) else 0, K,
-        wq.data_ptr(), N * w_row if Bw > 1 else 0, w_row, 1 if w_seg_as_batch else 0,
-        S, _Bounds(*bounds), int(group_size or 0), 1 if sw.dtype == torch.bfloat16 else 0,
-        sx.data_ptr(), sx_neg.data_ptr() if sx_neg is not None else None,
-        sx_strides[0] if sx_batch_stride is None else sx_batch_stride, sx_strides[1], sx_strides[2],
-        sw.data_ptr(), *sw_strides,
-        bias.data_ptr() if bias is not None else None, _dt(bias) if bias is not None else 0, 0, 0,
-        y.data_ptr(), y_bs, y_rs)
+    acc, peers, n_peers, prs, pco = None, _NO_PEERS, 0, 0, 0
     if peer_outputs is not None:
         # fused all-gather: (device pointers of the peers' [M, *] buffers, row stride, column offset) in elements
         ptrs, prs, pco = peer_outputs
-        if len(ptrs) > L.SQ_MAX_PEERS:
+        n_peers = len(ptrs)
+        if n_peers > L.SQ_MAX_PEERS:
             raise ValueError(f"at most {L.SQ_MAX_PEERS} peer outputs")
-        a.num_peer_outputs = len(ptrs)
-        for j, ptr in enumerate(ptrs):
-            a.peer_y_dev[j] = int(ptr)
-        a.peer_row_stride, a.peer_col_offset = int(prs), int(pco)
-    acc = None
+        peers = (*(int(ptr) for ptr in ptrs), *_NO_PEERS[n_peers:])
     if want_acc:
         units = num_units(bounds, group_size)
         sides = 2 if xq_neg is not None else 1
         acc = torch.zeros((batch, units, sides, M, N), dtype=torch.int32, device=xq.device)
-        a.acc_dump_dev = acc.data_ptr()
-    _run(L.load().sq_gemm, "sq_gemm", xq, ctypes.byref(a))
+    a = _GEMM.pack(
+        kind, _DT[out_dtype], batch, M, N, K,
+        xq.data_ptr(), xq_neg.data_ptr() if xq_neg is not None else 0, M * K if (x_batched and Bx > 1) else 0, K,
+        wq.data_ptr(), N * w_row if Bw > 1 else 0, w_row, 1 if w_seg_as_batch else 0,
+        S, struct.pack(f"{S + 1}i", *bounds), int(group_size or 0), 1 if sw.dtype == torch.bfloat16 else 0,
+        sx.data_ptr(), sx_neg.data_ptr() if sx_neg is not None else 0,
+        sx_strides[0] if sx_batch_stride is None else sx_batch_stride, sx_strides[1], sx_strides[2],
+        sw.data_ptr(), *sw_strides,
+        bias.data_ptr() if bias is not None else 0, _dt(bias) if bias is not None else 0, 0, 0,
+        y.data_ptr(), y_bs, y_rs, acc.data_ptr() if acc is not None else 0, n_peers, 0, *peers, int(prs), int(pco))
+    _run(L.load().sq_gemm, "sq_gemm", xq.get_device(), a)
     launch_count += 1
     return (y, acc) if want_acc else y
 
