@@ -156,7 +156,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     using C = AttnCfg<DP>;
     constexpr int ST = C::kStages;
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bar_q[2], bar_full[ST], bar_empty[ST], bar_s[2], bar_sfree[2], bar_p[2], bar_half[2], bar_pv[2], bar_tail;
+    __shared__ __align__(8) uint64_t bar_q[2], bar_full[ST], bar_empty[ST], bar_s[2], bar_sfree[2], bar_p[2], bar_pv[2], bar_tail;
     __shared__ AttnTile tile_s;
     __shared__ uint32_t tmem_s;
     __shared__ int abort_s;
@@ -180,7 +180,6 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 mbar_init(smem_u32(&bar_s[t]), 1);
                 mbar_init(smem_u32(&bar_sfree[t]), 4);
                 mbar_init(smem_u32(&bar_p[t]), 4);
-                mbar_init(smem_u32(&bar_half[t]), 4);
                 mbar_init(smem_u32(&bar_pv[t]), 1);
             }
             for (int s = 0; s < ST; ++s) {
@@ -272,16 +271,16 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             const int dk = (p.D + 15) & ~15;
             const uint32_t idesc_s = attn_idesc<T>(kAttnKeys, false), idesc_o = attn_idesc<T>(dk, true);
             const uint32_t b_full = smem_u32(&bar_full[0]), b_empty = smem_u32(&bar_empty[0]), b_q = smem_u32(&bar_q[0]), b_s = smem_u32(&bar_s[0]),
-                           b_sfree = smem_u32(&bar_sfree[0]), b_p = smem_u32(&bar_p[0]), b_half = smem_u32(&bar_half[0]), b_pv = smem_u32(&bar_pv[0]);
+                           b_sfree = smem_u32(&bar_sfree[0]), b_p = smem_u32(&bar_p[0]), b_pv = smem_u32(&bar_pv[0]);
             bool ok = true;
-            // two barriers at once: one round trip
-            auto wait2 = [&](uint32_t bar_a, uint32_t par_a, uint32_t bar_b, uint32_t par_b) {
+            // several barriers at once: one round trip, which takes 250 to 350 cycles next to the softmax warps
+            auto wait3 = [&](uint32_t bar_a, uint32_t par_a, uint32_t bar_b, uint32_t par_b, uint32_t bar_c, uint32_t par_c) {
                 if (!ok) return;
                 uint32_t it = 0;
                 long long t0 = 0;
                 for (;;) {
-                    const uint32_t ra = mbar_try_wait(bar_a, par_a), rb = mbar_try_wait(bar_b, par_b);
-                    if (__all_sync(0xffffffffu, ra & rb)) break;
+                    const uint32_t ra = mbar_try_wait(bar_a, par_a), rb = mbar_try_wait(bar_b, par_b), rc = mbar_try_wait(bar_c, par_c);
+                    if (__all_sync(0xffffffffu, ra & rb & rc)) break;
                     if ((it++ & 1023u) == 0u) {
                         if (it == 1u) t0 = clock64();
                         if (__any_sync(0xffffffffu, *abort_flag || clock64() - t0 > p.wait_cycles)) {
@@ -296,6 +295,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
                 tc_fence_after();
             };
+            auto wait2 = [&](uint32_t bar_a, uint32_t par_a, uint32_t bar_b, uint32_t par_b) { wait3(bar_a, par_a, bar_b, par_b, bar_b, par_b); };
             auto wait1 = [&](uint32_t bar, uint32_t par) { wait2(bar, par, bar, par); };
             // ring slot and lap of the next K and the next V tile (K and V lie in it in turn)
             int ks = 0, kl = 0, vs = 1, vl = 0;
@@ -319,23 +319,13 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     if (release) umma_commit(b_empty + ks * 8);
                 }
             };
-            // the product with the first half of P's keys, which is there while the softmax works on the second (DP = 128: the wait
-            // for the next S starts with this product)
-            auto product_half = [&](int t, uint32_t acc) {
-                const uint32_t b = (((sb + (2 + vs) * C::kTile) >> 4) & 0x3FFFu) | ((C::kHalf >> 4) << 16), a = tm + C::col_p(0) + t * (C::col_p(1) - C::col_p(0)),
-                               d = tm + C::col_o(0) + t * (C::col_o(1) - C::col_o(0));
-                if (leader) {
-#pragma unroll
-                    for (int k = 0; k < kAttnKeys / 32; ++k) mma_ts(d, a + k * 8, b + k * 128u, idesc_o, k > 0 ? 1u : acc);
-                }
-            };
             auto product_o = [&](int t, uint32_t acc, bool release) {
                 // rows of 64 columns: 8 keys are 1024 bytes (SBO), the next 64 columns kHalf bytes on (LBO)
                 const uint32_t b = (((sb + (2 + vs) * C::kTile) >> 4) & 0x3FFFu) | ((C::kHalf >> 4) << 16), a = tm + C::col_p(0) + t * (C::col_p(1) - C::col_p(0)),
                                d = tm + C::col_o(0) + t * (C::col_o(1) - C::col_o(0));
                 if (leader) {
 #pragma unroll
-                    for (int k = C::kOwnP ? 0 : kAttnKeys / 32; k < kAttnKeys / 16; ++k) mma_ts(d, a + k * 8, b + k * 128u, idesc_o, k > 0 ? 1u : acc);
+                    for (int k = 0; k < kAttnKeys / 16; ++k) mma_ts(d, a + k * 8, b + k * 128u, idesc_o, k > 0 ? 1u : acc);
                     umma_commit(b_pv + t * 8);
                     if (release) umma_commit(b_empty + vs * 8);
                 }
@@ -377,15 +367,12 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 for (int j = 0; ok && j < nn; ++j) {
                     const bool more = j + 1 < nn;
                     const int kb = more ? ks : vs, kp = more ? kl : vl;
-                    wait2(b_full + vs * 8, vl, b_full + kb * 8, kp);
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         const int nt = t ? n1 : n0;
                         if (ok && j < nt) {
-                            wait1(b_half + t * 8, j & 1u);
-                            if (ok) product_half(t, j > 0);
-                            wait1(b_p + t * 8, j & 1u);
-                            if (ok) product_o(t, 1, t == 1 || j >= n1);
+                            wait3(b_p + t * 8, j & 1u, b_full + vs * 8, vl, b_full + kb * 8, kp);
+                            if (ok) product_o(t, j > 0, t == 1 || j >= n1);
                             if (ok && j + 1 < nt) product_s(t, t == 1 || j + 1 >= n1);
                         }
                     }
@@ -423,7 +410,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         // keys that every row of this warp sees (rows that are not stored do not count): no comparison needed below it
         const int seen_by_all = __reduce_min_sync(0xffffffffu, mine ? limit : 0x7fffffff);
         const int nt = t ? n_sub[1] : n_sub[0];
-        const uint32_t bs = smem_u32(&bar_s[t]), bsf = smem_u32(&bar_sfree[t]), bp = smem_u32(&bar_p[t]), bh = smem_u32(&bar_half[t]), bpv = smem_u32(&bar_pv[t]);
+        const uint32_t bs = smem_u32(&bar_s[t]), bsf = smem_u32(&bar_sfree[t]), bp = smem_u32(&bar_p[t]), bpv = smem_u32(&bar_pv[t]);
         const float c = p.scale_log2;
         const int cols = (p.D + 15) & ~15;
         float m_ref = -INFINITY, l = 0.0f;
@@ -515,12 +502,6 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 if (i == 31) {
                     wait_pv();
                     tmem_st_x32(tp, pk);
-                    if constexpr (!C::kOwnP) {
-                        tmem_st_wait_all();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(bh);
-                    }
                 }
             }
             pass_turn(j);
