@@ -9,6 +9,13 @@
 //   warp 9         : issues tcgen05.mma: S = q k^T (both operands in shared memory), O += P v (P in tensor memory)
 //   warp 10        : clears the rows behind the last key in the last v tile (what lies there may be NaN, and 0 * NaN is NaN)
 //
+// What bounds it.  A pair of 128 x 128 tiles takes 1100 (heads of 64) or 2048 (128) cycles of products and 2048 of
+// exponentials, less what the FMA pipe takes over; the loop needs 2700 and 3400.  Heads of 64: softmax and products run side by
+// side, 332 us = 726 TFLOP/s at the size above (the exponentials alone would take 215 us, the products 144).  Heads of 128: tensor
+// memory holds one S a sub-tile, so softmax, O and the next S follow one another within a sub-tile and only the two
+// sub-tiles overlap, 494 us = 1250 TFLOP/s at 12288 causal tokens, 16 query heads on 2 (products 368 us).  A cluster of
+// CTAs that shared k and v would save L2 traffic that bounds nothing (85 to 92 % hits, DRAM 2 to 3 %).
+//
 // One pass over the keys with a running maximum m and sum l per row: p = 2^(c (s - m)), O and l are scaled by
 // 2^(c (m_old - m_new)) when the maximum grows.  O lives in tensor memory and is only rescaled when a row's maximum has
 // grown by more than 2^8 since the last time (every p then stays below 2^8, well inside fp32 sums and fp16 p); the result
@@ -31,7 +38,9 @@ enum AttnWait : int { kAttnMma = 20, kAttnKvEmpty = 22, kAttnS = 23, kAttnPv = 2
 
 constexpr int kAttnThreads = 384;
 // Of kPolyOf pairs of exponentials, kPoly go to the FMA pipe (ex2_poly).  The special-function pipe does 4 lanes a cycle: two
-// warps' 128 exponentials a row take 2048 cycles there while everything else that a tile needs takes about 1000.
+// warps' 128 exponentials a row take 2048 cycles there while everything else that a tile needs takes about 1000.  4429 tokens,
+// 24 heads of 64, two samples: none 361 us, one of eight 335, one of six 332, one of four 347 (the other pipes and the issue
+// slots fill up); 128 wide heads do not care (507, 505, 504, 507 us at 12288 causal tokens).
 constexpr int kPoly = 1, kPolyOf = 6;
 constexpr int kWarpMma = 9;         // and the next one
 constexpr int kAttnRows = 128;       // rows of a sub-tile = tensor-memory lanes

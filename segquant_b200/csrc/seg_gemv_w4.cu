@@ -10,8 +10,12 @@
 // columns in flight; nothing waits for another warp), a word of 8 nibbles becomes two words of bytes 16 * q (even and odd
 // columns) with a shift and two masks, and since the order of the inner dimension is free, the activations wait in shared
 // memory with the even and the odd bytes of every 8 columns side by side.  An output lives in one lane from the first unit to
-// the last, so the fp32 sum over the units runs in registers.  Dot products on the ALUs (dp4a) were measured first: 72 us at
-// 16384 x 12288 with 4 rows against 147 us on the 128-row tiles; the conversions, shuffles and sums around them bound it.
+// the last, so the fp32 sum over the units runs in registers.
+//
+// 16384 x 12288, groups of 128, 4 rows (98 MB of weights, floor 16 us): 42 us, 147 us on the 128-row tiles.  7 warps an SM walk
+// 96 blocks each, some 150 instructions a block, and that chain bounds it (without groups, 28 us).  Measured and not kept:
+// dot products on the ALUs (dp4a) 72 us; two blocks a step 51; scales through the ring 43; closing a unit a block later 43;
+// tiles of 8 columns on twice the warps 48; three warps to a tile that exchange their integer sums 42 to 52.
 #include <cstdlib>
 
 #include "seg_gemm_params.cuh"
