@@ -6,14 +6,15 @@
 //
 //   warps 0-3, 4-7 : softmax of sub-tile 0 / 1, one row per thread
 //   warp 8         : TMA loads (q once, k and v through a ring of stages)
-//   warp 9         : issues tcgen05.mma: S = q k^T (both operands in shared memory), O += P v (P in tensor memory)
-//   warp 10        : clears the rows behind the last key in the last v tile (what lies there may be NaN, and 0 * NaN is NaN)
+//   warp 9 (, 10)  : issue tcgen05.mma: S = q k^T (both operands in shared memory), O += P v (P in tensor memory); heads up to
+//                    64 wide have a warp for each sub-tile
+//   warp 11        : clears the rows behind the last key in the last v tile (what lies there may be NaN, and 0 * NaN is NaN)
 //
 // What bounds it.  A pair of 128 x 128 tiles takes 1100 (heads of 64) or 2048 (128) cycles of products and 2048 of
 // exponentials, less what the FMA pipe takes over; the loop needs 2700 and 3400.  Heads of 64: softmax and products run side by
-// side, 332 us = 726 TFLOP/s at the size above (the exponentials alone would take 215 us, the products 144).  Heads of 128: tensor
+// side, 332 us = 726 TFLOP/s for two samples of 4429 tokens, 24 heads (the exponentials alone would take 202 us, the products 144).  Heads of 128: tensor
 // memory holds one S a sub-tile, so softmax, O and the next S follow one another within a sub-tile and only the two
-// sub-tiles overlap, 494 us = 1250 TFLOP/s at 12288 causal tokens, 16 query heads on 2 (products 368 us).  A cluster of
+// sub-tiles overlap, 494 to 504 us = 1227 to 1250 TFLOP/s at 12288 causal tokens, 16 query heads on 2 (products 368 us).  A cluster of
 // CTAs that shared k and v would save L2 traffic that bounds nothing (85 to 92 % hits, DRAM 2 to 3 %).
 //
 // One pass over the keys with a running maximum m and sum l per row: p = 2^(c (s - m)), O and l are scaled by
@@ -42,7 +43,7 @@ constexpr int kAttnThreads = 384;
 // 24 heads of 64, two samples: none 361 us, one of eight 335, one of six 332, one of four 347 (the other pipes and the issue
 // slots fill up); 128 wide heads do not care (507, 505, 504, 507 us at 12288 causal tokens).
 constexpr int kPoly = 1, kPolyOf = 6;
-constexpr int kWarpMma = 9;         // and the next one
+constexpr int kWarpMma = 9;         // and the next one with heads up to 64 wide
 constexpr int kAttnRows = 128;       // rows of a sub-tile = tensor-memory lanes
 constexpr int kAttnKeys = 128;       // keys of a tile
 

@@ -6,8 +6,8 @@
 // Angles of far positions lose everything in fp32 (position 10^5 leaves 2^-7 of a radian), so the turn is counted in
 // revolutions in fp64, reduced to [-1/2, 1/2] there and only then rounded: one fp64 multiplication per (token, pair).  A
 // thread keeps the sines of its columns in registers and walks the heads, which share them.  Everything else is fp32 with
-// one rounding at the end.  32760 tokens, 16 + 16 heads of 128, fp16: 86 us = 6.25 TB/s (copy 6.55); 2 x 4429 tokens, 24 + 24
-// heads of 64 behind their normalisation: 24 us = 4.6 TB/s, two and a half rounds of CTAs and the sines of each.
+// one rounding at the end.  32760 tokens, 16 + 16 heads of 128, fp16: 87 us = 6.2 TB/s (copy 6.55); 2 x 4429 tokens, 24 + 24
+// heads of 64 behind their normalisation: 24 us = 4.6 TB/s, 2.8 rounds of CTAs and the sines of each.
 #include <cmath>
 #include <type_traits>
 
