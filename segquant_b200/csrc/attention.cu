@@ -531,7 +531,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             tc_fence_after();
         }
         if (ok && live[t]) {
-            const bool empty = m_ref == -INFINITY && l == l;     // no key seen (the polynomial's 2^-126 does not count)
+            const bool empty = m_ref == -INFINITY && l == l;     // no key seen
             const float inv = empty ? 0.0f : 1.0f / l;
             const float lse2 = empty ? -INFINITY : m_ref * c + log2f(l);
             const long long token = static_cast<long long>(T0.b) * (p.q_off ? 0 : p.Tq) + T0.q_base + tok;

@@ -142,13 +142,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {      // NaN c
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
 }
-// 2^x of two values on the FMA pipe, for x in [-inf, 100] (2^-126 below -126) or NaN: x = n + f with n the nearest whole
-// number, 2^n from the low bits of x + 1.5 * 2^23 + 127 (which are those of n + 127) and 2^f from a polynomial of degree 4,
-// 1 + c1 f + ..., fitted to the least largest relative error on [-1/2, 1/2] (3e-6; a cubic, 1e-4, is enough for the 16-bit p,
-// but shows in the logarithm of a short row's sum).  2^0 is exactly 1.
+// 2^x of two values on the FMA pipe, for x in [-inf, 100] or NaN (0 below -126.5, so that masked keys weigh nothing):
+// x = n + f with n the nearest whole number, 2^n from the low bits of x + 1.5 * 2^23 + 127 (which are those of n + 127; n = -127
+// leaves an exponent field of zero: 0) and 2^f from a polynomial of degree 4, 1 + c1 f + ..., fitted to the least largest
+// relative error on [-1/2, 1/2] (3e-6; a cubic, 1e-4, is enough for the 16-bit p, but shows in the logarithm of a short row's
+// sum).  2^0 is exactly 1.
 __device__ __forceinline__ float2 ex2_poly(float2 x) {
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-126.0f));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-126.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.x) : "f"(-127.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x.y) : "f"(-127.0f));
     const float2 big = make_float2(12583039.0f, 12583039.0f), nbig = make_float2(-12583039.0f, -12583039.0f);
     const float2 t = __fadd2_rn(x, big);
     const float2 n = __fadd2_rn(t, nbig);

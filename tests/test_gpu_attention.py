@@ -308,3 +308,16 @@ def test_refusals(native_lib):
             pytest.fail(f"call {i} was not refused")
     with torch.no_grad():
         ops.attention(x.clone().requires_grad_(), x, x)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("tq,d", [(256, 64), (256, 128), (300, 40), (4, 64)])
+def test_hidden_values_weigh_nothing(native_lib, dtype, tq, d):
+    """Keys that causality hides have weight 0 exactly, whatever finite value they carry (2^-126 times the largest bf16 is 4)."""
+    g = torch.Generator(device="cuda").manual_seed(tq + d)
+    q, k, v = (torch.randn(1, tq, 2, d, generator=g, device="cuda").to(dtype) for _ in range(3))
+    half = tq // 2
+    big = v.clone()
+    big[:, half:] = torch.finfo(dtype).max
+    clean, hidden = ops.attention(q, k, v, causal=True), ops.attention(q, k, big, causal=True)
+    assert torch.equal(clean[:, :half], hidden[:, :half])
