@@ -6,8 +6,8 @@
 // Angles of far positions lose everything in fp32 (position 10^5 leaves 2^-7 of a radian), so the turn is counted in
 // revolutions in fp64, reduced to [-1/2, 1/2] there and only then rounded: one fp64 multiplication per (token, pair).  A
 // thread keeps the sines of its columns in registers and walks the heads, which share them.  Everything else is fp32 with
-// one rounding at the end.  32760 tokens, 16 + 16 heads of 128, fp16: 87 us = 6.2 TB/s (copy 6.55); 2 x 4429 tokens, 24 + 24
-// heads of 64 behind their normalisation: 24 us = 4.6 TB/s, 2.8 rounds of CTAs and the sines of each.
+// one rounding at the end.  32760 tokens, 16 + 16 heads of 128, fp16: 85 us = 6.3 TB/s (copy 6.55); 2 x 4429 tokens, 24 + 24
+// heads of 64 behind their normalisation: 22 us = 5.0 TB/s, 1.9 rounds of CTAs and the sines of each.
 #include <cmath>
 #include <type_traits>
 
@@ -26,7 +26,7 @@ struct RotaryParams {
     const void* pos;
     long long pos_bs, pos_ts;
     long long batch, tokens;          // tokens of one batch entry
-    int D, pairs;                     // rotated pairs
+    int D, pairs, all_pairs;          // rotated pairs; scalar kernel: and those of the columns behind the axes
     int pos_float, halves;
     int heads_per_cta;                // heads (of q, then of k) that one CTA's threads walk
     int group;                        // vector kernel: threads that share a row (power of two)
@@ -114,8 +114,16 @@ struct RotRow {                       // 8 columns as loaded
 constexpr int kRotAhead = 4;
 constexpr int kRotThreads = 128;
 constexpr int kRotWarps = 32;          // per SM; 48 to 96 measured the same or slower (64 x 64 grid, two samples: 23.8 against 24.4 to 26.0 us)
+// CTAs that an SM has room for: what bounds the registers, and with them the loads in flight.  Adjacent pairs, image tokens (2 x 4429,
+// 24 + 24 heads of 64 behind their normalisation) and clip (32760 tokens, 32 heads of 128): unbounded 24.2 and 86.5 us, five 23.1
+// and 85.9, six 21.9 and 85.3, eight 26 (spills).  Halves, the same tokens: 16-bit 24.6 and 89.7 us with five, 97 with four or fewer, 93 with
+// six; behind the normalisation 25.0 and 98.7 with four, 27.0 and 98.3 with five, 30 and 109 with three; fp32 47 and 182 with three,
+// 45 and 202 with four.
 template <typename T, bool HALVES, bool NORM>
-__global__ void __launch_bounds__(kRotThreads) rotary_vec_kernel(const __grid_constant__ RotaryParams p) {
+constexpr int rot_vec_ctas() { return !HALVES ? 6 : sizeof(T) == 4 ? 3 : NORM ? 4 : 5; }
+
+template <typename T, bool HALVES, bool NORM>
+__global__ void __launch_bounds__(kRotThreads, (rot_vec_ctas<T, HALVES, NORM>())) rotary_vec_kernel(const __grid_constant__ RotaryParams p) {
     constexpr int NV = HALVES ? 2 : 1;
     constexpr int U = (sizeof(T) == 4 || HALVES) ? kRotAhead / 2 : kRotAhead;
     const int u = threadIdx.x & (p.group - 1);
@@ -235,69 +243,112 @@ __global__ void __launch_bounds__(kRotThreads) rotary_vec_kernel(const __grid_co
     }
 }
 
-// Any width, stride and alignment: one warp per token, lane l has the pairs l, l + 32, ... and walks heads.
-template <typename T, bool NORM>
-__global__ void __launch_bounds__(kRotThreads) rotary_scalar_kernel(const __grid_constant__ RotaryParams p) {
-    constexpr int NP = kRotMaxPairs / 32;
+// Any width, stride and alignment: one warp per token, lane l has the pairs l, l + 32, ... and walks heads, 8 / NP at a time (all
+// their loads are out before the first store, which the compiler could not move them across).  Columns behind the axes are
+// pairs that are not turned, the last of them alone (step 0) if their number is odd.  Halves of 28 columns, the clip's 32760 tokens,
+// 32 heads of 128: 16-bit 229 us (a head at a time 981; 333 with the registers unbounded), behind the normalisation 279 (1000); fp32
+// 216 (981; 258 when bounded to eight CTAs an SM), 293 (998).
+template <typename T, bool NORM, int NP>
+__global__ void __launch_bounds__(kRotThreads, sizeof(T) == 4 ? 0 : 8) rotary_scalar_kernel(const __grid_constant__ RotaryParams p) {
+    constexpr int U = 8 / NP;
     const int lane = threadIdx.x & 31;
     const long long row = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
     if (row >= p.batch * p.tokens) return;
     const long long b = row / p.tokens, t = row - b * p.tokens;
     const bool halves = p.halves != 0;
     float cs[NP], sn[NP];
+    int ca[NP], cc[NP];
+    bool has[NP], two[NP], turned[NP];
 #pragma unroll
-    for (int i = 0; i < NP; ++i)
-        if (lane + 32 * i < p.pairs) {
-            const float2 a = rot_angle(p, b, t, lane + 32 * i);
-            cs[i] = a.x;
-            sn[i] = a.y;
-        }
-    const int h0 = blockIdx.y * p.heads_per_cta, h1 = min(h0 + p.heads_per_cta, p.heads[0] + p.heads[1]);
-    for (int hh = h0; hh < h1; ++hh) {
-        const int part = hh >= p.heads[0], h = part ? hh - p.heads[0] : hh;
-        const T* x = static_cast<const T*>(p.x[part]) + b * p.x_bs[part] + t * p.x_ts[part] + h * p.x_hs[part];
-        T* y = static_cast<T*>(p.y[part]) + b * p.y_bs[part] + t * p.y_ts[part] + h * p.y_hs[part];
-        const T* w = static_cast<const T*>(p.weight[part]);
-        float r = 1.0f;
-        if constexpr (NORM) {
-            float ss = 0.0f;
-            for (int i = lane; i < p.D; i += 32) {
-                const float v = to_float<T>(x[i]);
-                ss = fmaf(v, v, ss);
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            r = rsqrtf(ss * p.inv_d + p.eps);
-        }
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int pair = lane + 32 * i;
-            if (pair < p.pairs) {
-                const int a = p.col[pair], c = a + p.step[pair];
-                float u = to_float<T>(x[a]), v = to_float<T>(x[c]);
-                if constexpr (NORM) {
-                    u *= r * to_float<T>(w[a]);
-                    v *= r * to_float<T>(w[c]);
-                }
-                // the vector kernel's products and sums, so that a layout does not show in the result
-                y[a] = from_float<T>(fmaf(u, cs[i], __fmul_rn(v, -sn[i])));
-                y[c] = from_float<T>(halves ? fmaf(u, sn[i], __fmul_rn(v, cs[i])) : fmaf(v, cs[i], __fmul_rn(u, sn[i])));
-            }
-        }
-        for (int i = 2 * p.pairs + lane; i < p.D; i += 32) {
-            float v = to_float<T>(x[i]);
-            if constexpr (NORM) v *= r * to_float<T>(w[i]);
-            y[i] = from_float<T>(v);
-        }
-        __syncwarp();
+    for (int n = 0; n < NP; ++n) {
+        const int pair = lane + 32 * n;
+        has[n] = pair < p.all_pairs;
+        turned[n] = pair < p.pairs;
+        ca[n] = has[n] ? p.col[pair] : 0;
+        cc[n] = has[n] ? ca[n] + p.step[pair] : 0;
+        two[n] = cc[n] != ca[n];
+        const float2 a = turned[n] ? rot_angle(p, b, t, pair) : make_float2(1.0f, 0.0f);
+        cs[n] = a.x;
+        sn[n] = a.y;
     }
+    const int h0 = blockIdx.y * p.heads_per_cta, h1 = min(h0 + p.heads_per_cta, p.heads[0] + p.heads[1]);
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+        const int first = part ? max(h0 - p.heads[0], 0) : h0, last = part ? h1 - p.heads[0] : min(h1, p.heads[0]);
+        if (first >= last) continue;
+        const long long xs = p.x_hs[part], ys = p.y_hs[part];
+        const T* x = static_cast<const T*>(p.x[part]) + b * p.x_bs[part] + t * p.x_ts[part] + first * xs;
+        T* y = static_cast<T*>(p.y[part]) + b * p.y_bs[part] + t * p.y_ts[part] + first * ys;
+        const T* w = static_cast<const T*>(p.weight[part]);
+        float wa[NP], wc[NP];
+        if constexpr (NORM) {
+#pragma unroll
+            for (int n = 0; n < NP; ++n) {
+                wa[n] = has[n] ? to_float<T>(w[ca[n]]) : 0.0f;
+                wc[n] = two[n] ? to_float<T>(w[cc[n]]) : 0.0f;
+            }
+        }
+        for (int h = first; h < last; h += U, x += U * xs, y += U * ys) {
+            float u[U][NP], v[U][NP];
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+#pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    const bool in = h + i < last;
+                    u[i][n] = in && has[n] ? to_float<T>(x[i * xs + ca[n]]) : 0.0f;
+                    v[i][n] = in && two[n] ? to_float<T>(x[i * xs + cc[n]]) : 0.0f;
+                }
+            if constexpr (NORM) {
+                float ss[U];
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    ss[i] = 0.0f;
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) ss[i] = fmaf(v[i][n], v[i][n], fmaf(u[i][n], u[i][n], ss[i]));
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+                    for (int i = 0; i < U; ++i) ss[i] += __shfl_xor_sync(0xffffffffu, ss[i], o);
+#pragma unroll
+                for (int i = 0; i < U; ++i) {
+                    const float r = rsqrtf(ss[i] * p.inv_d + p.eps);
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) {
+                        u[i][n] *= r * wa[n];
+                        v[i][n] *= r * wc[n];
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+#pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    if (h + i >= last || !has[n]) continue;
+                    float ya = u[i][n], yc = v[i][n];
+                    if (turned[n]) {      // the vector kernel's products and sums, so that a layout does not show in the result
+                        ya = fmaf(u[i][n], cs[n], __fmul_rn(v[i][n], -sn[n]));
+                        yc = halves ? fmaf(u[i][n], sn[n], __fmul_rn(v[i][n], cs[n])) : fmaf(v[i][n], cs[n], __fmul_rn(u[i][n], sn[n]));
+                    }
+                    y[i * ys + ca[n]] = from_float<T>(ya);
+                    if (two[n]) y[i * ys + cc[n]] = from_float<T>(yc);
+                }
+        }
+    }
+}
+
+template <typename T, bool NORM>
+static void launch_rotary_scalar(const RotaryParams& p, dim3 grid, cudaStream_t st) {
+    if (p.all_pairs <= 32) rotary_scalar_kernel<T, NORM, 1><<<grid, kRotThreads, 0, st>>>(p);
+    else if (p.all_pairs <= 64) rotary_scalar_kernel<T, NORM, 2><<<grid, kRotThreads, 0, st>>>(p);
+    else rotary_scalar_kernel<T, NORM, kRotMaxPairs / 32><<<grid, kRotThreads, 0, st>>>(p);
 }
 
 template <typename T>
 static void launch_rotary(const RotaryParams& p, bool vec, bool halves, bool norm, dim3 grid, cudaStream_t st) {
     if (!vec) {
-        if (norm) rotary_scalar_kernel<T, true><<<grid, kRotThreads, 0, st>>>(p);
-        else rotary_scalar_kernel<T, false><<<grid, kRotThreads, 0, st>>>(p);
+        if (norm) launch_rotary_scalar<T, true>(p, grid, st);
+        else launch_rotary_scalar<T, false>(p, grid, st);
     } else if (halves) {
         if (norm) rotary_vec_kernel<T, true, true><<<grid, kRotThreads, 0, st>>>(p);
         else rotary_vec_kernel<T, true, false><<<grid, kRotThreads, 0, st>>>(p);
@@ -377,7 +428,11 @@ int rotary(const sq_rotary_args* a, cudaStream_t st) {
     }
     p.pos = a->positions_dev; p.pos_float = a->positions_float ? 1 : 0; p.halves = halves ? 1 : 0;
     p.pos_bs = a->pos_batch_stride; p.pos_ts = a->pos_token_stride;
-    p.batch = a->batch; p.tokens = a->tokens; p.D = a->D; p.pairs = width / 2; p.eps = a->eps; p.inv_d = 1.0f / static_cast<float>(a->D);
+    p.batch = a->batch; p.tokens = a->tokens; p.D = a->D; p.pairs = width / 2; p.all_pairs = p.pairs; p.eps = a->eps; p.inv_d = 1.0f / static_cast<float>(a->D);
+    for (int c = width; c < a->D; c += 2, ++p.all_pairs) {
+        p.col[p.all_pairs] = static_cast<short>(c);
+        p.step[p.all_pairs] = c + 1 < a->D ? 1 : 0;
+    }
     p.units = units;
     p.group = 1;
     while (p.group < units) p.group *= 2;

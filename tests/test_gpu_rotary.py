@@ -150,3 +150,35 @@ def test_nothing_to_do_and_refusals(native_lib):
         with pytest.raises(kind):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("hq,hk,d,axes,pairing", [(9, 17, 33, (6, 10), "halves"), (5, 3, 100, (20, 22, 22), "halves"), (11, 2, 251, (80, 90, 80), "adjacent"),
+                                                 (7, 9, 129, (128,), "halves")])
+def test_odd_layouts_in_place(native_lib, hq, hk, d, axes, pairing, norm, dtype):
+    """Views that start at an odd element, heads that no step of several divides, written in place; what lies between them stays."""
+    g = _gen(11)
+    buf = torch.randn(2, 37, hq + hk, d + 3, generator=g, device=DEV).to(dtype)
+    before = buf.clone()
+    cut = lambda t: (t[:, :, :hq, 1:d + 1], t[:, :, hq:, 1:d + 1])  # noqa: E731
+    q, k = cut(buf)
+    pos = torch.randint(0, 500, (37, len(axes)), generator=g, device=DEV, dtype=torch.int32)
+    w = [torch.randn(d, generator=g, device=DEV).to(dtype) for _ in range(2)] if norm else [None, None]
+    ops.rotary(q, k, pos, axes, pairing=pairing, norm_q=w[0], norm_k=w[1], out_q=q, out_k=k)
+    for got, x, weight in zip(cut(buf), cut(before), w):
+        _check(got, x, pos[None], axes, 10000.0, pairing, weight)
+    assert torch.equal(buf[..., 0], before[..., 0]) and torch.equal(buf[..., d + 1:], before[..., d + 1:])
+
+
+def test_columns_behind_the_axes_are_not_mixed(native_lib):
+    x = torch.randn(1, 6, 3, 51, generator=_gen(12), device=DEV)
+    bad = x.clone()
+    bad[..., 41], bad[..., 50] = float("nan"), float("inf")
+    pos = torch.arange(6, device=DEV, dtype=torch.int32)[:, None]
+    out = lambda t: ops.rotary(t, t, pos, (40,))[0]  # noqa: E731
+    clean, got = out(x), out(bad)
+    keep = torch.ones(51, dtype=torch.bool, device=DEV)
+    keep[41] = keep[50] = False
+    assert torch.equal(clean[..., keep], got[..., keep]) and torch.isnan(got[..., 41]).all() and torch.isinf(got[..., 50]).all()
+    assert torch.equal(clean[..., 40:], x[..., 40:])
