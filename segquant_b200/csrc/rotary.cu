@@ -122,7 +122,8 @@ constexpr int kRotWarps = 32;          // per SM; 48 to 96 measured the same or 
 template <typename T, bool HALVES, bool NORM>
 constexpr int rot_vec_ctas() { return !HALVES ? 6 : sizeof(T) == 4 ? 3 : NORM ? 4 : 5; }
 
-template <typename T, bool HALVES, bool NORM>
+// REST: there are columns behind the axes (a form of its own: the selects cost the other one registers, image tokens 20.5 -> 21.2 us).
+template <typename T, bool HALVES, bool NORM, bool REST>
 __global__ void __launch_bounds__(kRotThreads, (rot_vec_ctas<T, HALVES, NORM>())) rotary_vec_kernel(const __grid_constant__ RotaryParams p) {
     constexpr int NV = HALVES ? 2 : 1;
     constexpr int U = (sizeof(T) == 4 || HALVES) ? kRotAhead / 2 : kRotAhead;
@@ -226,6 +227,16 @@ __global__ void __launch_bounds__(kRotThreads, (rot_vec_ctas<T, HALVES, NORM>())
                         o[NV - 1][k] = __ffma2_rn(e[i][0][k], sn[k], __fmul2_rn(e[i][NV - 1][k], cs[k]));
                     } else {
                         o[0][k] = __ffma2_rn(e[i][0][k], cs[k], __fmul2_rn(make_float2(e[i][0][k].y, e[i][0][k].x), sn[k]));
+                    }
+                }
+                if constexpr (REST) {     // these columns stay: 1 * y + 0 * partner would pass the partner's NaN or infinity on
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if constexpr (HALVES) {
+                            if (pair0 < 0) { o[0][k] = e[i][0][k]; o[NV - 1][k] = e[i][NV - 1][k]; }
+                        } else if (pair0 + k >= p.pairs) {
+                            o[0][k] = e[i][0][k];
+                        }
                     }
                 }
                 if (has && h + i < last) {
@@ -344,17 +355,26 @@ static void launch_rotary_scalar(const RotaryParams& p, dim3 grid, cudaStream_t 
     else rotary_scalar_kernel<T, NORM, kRotMaxPairs / 32><<<grid, kRotThreads, 0, st>>>(p);
 }
 
+template <typename T, bool REST>
+static void launch_rotary_vec(const RotaryParams& p, bool halves, bool norm, dim3 grid, cudaStream_t st) {
+    if (halves) {
+        if (norm) rotary_vec_kernel<T, true, true, REST><<<grid, kRotThreads, 0, st>>>(p);
+        else rotary_vec_kernel<T, true, false, REST><<<grid, kRotThreads, 0, st>>>(p);
+    } else {
+        if (norm) rotary_vec_kernel<T, false, true, REST><<<grid, kRotThreads, 0, st>>>(p);
+        else rotary_vec_kernel<T, false, false, REST><<<grid, kRotThreads, 0, st>>>(p);
+    }
+}
+
 template <typename T>
 static void launch_rotary(const RotaryParams& p, bool vec, bool halves, bool norm, dim3 grid, cudaStream_t st) {
     if (!vec) {
         if (norm) launch_rotary_scalar<T, true>(p, grid, st);
         else launch_rotary_scalar<T, false>(p, grid, st);
-    } else if (halves) {
-        if (norm) rotary_vec_kernel<T, true, true><<<grid, kRotThreads, 0, st>>>(p);
-        else rotary_vec_kernel<T, true, false><<<grid, kRotThreads, 0, st>>>(p);
+    } else if (2 * p.pairs < p.D) {
+        launch_rotary_vec<T, true>(p, halves, norm, grid, st);
     } else {
-        if (norm) rotary_vec_kernel<T, false, true><<<grid, kRotThreads, 0, st>>>(p);
-        else rotary_vec_kernel<T, false, false><<<grid, kRotThreads, 0, st>>>(p);
+        launch_rotary_vec<T, false>(p, halves, norm, grid, st);
     }
 }
 
