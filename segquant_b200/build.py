@@ -19,7 +19,7 @@ SOURCES = ["capi.cu", "act_quant.cu", "weight_quant.cu", "seg_gemm.cu", "seg_gem
            # one translation unit per (kind, DualScale): the GEMM kernels dominate compile time and build in parallel
            "seg_gemm_tu_i8.cu", "seg_gemm_tu_i8_dual.cu", "seg_gemm_tu_f8.cu", "seg_gemm_tu_f8_dual.cu",
            "seg_gemm_tu_w4.cu", "seg_gemm_tu_w4_dual.cu"]
-HEADERS = [os.path.join(CSRC, h) for h in ("common.cuh", "ptx.cuh", "attention.cuh", "seg_gemm_params.cuh", "seg_gemm_kernels.cuh", "seg_gemm_2cta.cuh",
+HEADERS = [os.path.join(CSRC, h) for h in ("common.cuh", "ptx.cuh", "attention.cuh", "attention_turns.cuh", "seg_gemm_params.cuh", "seg_gemm_kernels.cuh", "seg_gemm_2cta.cuh",
                                            "seg_gemm_epilogue.cuh")] + [os.path.join(PKG_DIR, "..", "include", "segquant_b200.h")]
 
 NVCC_FLAGS = [

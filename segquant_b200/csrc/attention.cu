@@ -26,6 +26,7 @@
 #include <cudaTypedefs.h>
 
 #include "attention.cuh"
+#include "attention_turns.cuh"
 #include "ptx.cuh"
 
 namespace sq {
@@ -127,6 +128,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
         ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kSmemDescHi)
         : "memory");
 }
+// barriers of AttnTurns: named barriers of two warps
+struct TurnBarrier {
+    int mine, other;
+    __device__ __forceinline__ void sync() { asm volatile("bar.sync %0, 64;" ::"r"(mine) : "memory"); }
+    __device__ __forceinline__ void arrive() { asm volatile("bar.arrive %0, 64;" ::"r"(other) : "memory"); }
+};
 __device__ __forceinline__ void tmem_st_wait_all() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Head widths up to DP (64 or 128): narrower heads are filled up with zeros by the TMA loads.
@@ -394,7 +401,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         } else if (warp == kWarpMma + 2 && tail) {
             // ------------------------------------------------------------------ rows behind the last key
             const int s = (2 * n - 1) % ST;
-            if (mbar_wait(smem_u32(&bar_tail), 0, abort_flag, kAttnTail, p.wait_cycles)) {
+            if (mbar_wait_warp(smem_u32(&bar_tail), 0, abort_flag, kAttnTail, p.wait_cycles)) {
                 const int valid = T0.kv_len - (lo + n - 1) * kAttnKeys;
                 uint8_t* v = smem + (2 + s) * C::kTile;
                 for (int h = 0; h < DP / 64; ++h)
@@ -426,16 +433,13 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         float m_ref = -INFINITY, l = 0.0f;
         bool ok = true;
         // The two warps of an SM quarter (one of each sub-tile) take turns with their exponentials: while one fills the
-        // special-function pipe the other loads, compares and stores.  A warp that gives up still passes its turns on.
-        const int turns = min(n_sub[0], n_sub[1]);
-        const int my_turn = 1 + t * 4 + (warp & 3), other_turn = 1 + (t ^ 1) * 4 + (warp & 3);
-        auto pass_turn = [&](int j) {
-            if (j + t < turns) asm volatile("bar.arrive %0, 64;" ::"r"(other_turn) : "memory");
-        };
-        if (t == 1 && turns > 0) asm volatile("bar.arrive %0, 64;" ::"r"(other_turn) : "memory");
+        // special-function pipe the other loads, compares and stores.
+        AttnTurns<TurnBarrier> turn = {{1 + t * 4 + (warp & 3), 1 + (t ^ 1) * 4 + (warp & 3)}, min(n_sub[0], n_sub[1]), t};
+        auto wait = [&](uint32_t bar, uint32_t parity, int code) { return mbar_wait_warp(bar, parity, abort_flag, code, p.wait_cycles); };
+        turn.open();
         int j = 0;
         for (; j < nt; ++j) {
-            if (!mbar_wait(bs, j & 1u, abort_flag, kAttnS, p.wait_cycles)) { ok = false; break; }
+            if (!wait(bs, j & 1u, kAttnS)) { ok = false; break; }
             tc_fence_after();
             uint32_t s[128];
             const int key0 = (lo + j) * kAttnKeys;
@@ -472,7 +476,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             auto wait_pv = [&]() {
                 if (!pv_done) {
                     pv_done = true;
-                    if (!mbar_wait(bpv, (j - 1) & 1u, abort_flag, kAttnPv, p.wait_cycles)) ok = false;
+                    if (!wait(bpv, (j - 1) & 1u, kAttnPv)) ok = false;
                     tc_fence_after();
                 }
             };
@@ -493,7 +497,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     }
                 }
             }
-            if (j < turns) asm volatile("bar.sync %0, 64;" ::"r"(my_turn) : "memory");
+            turn.take(j);
             const float mc = m_ref == -INFINITY ? 0.0f : m_ref * c;
             const float2 c2 = make_float2(c, c), mc2 = make_float2(-mc, -mc);
             float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
@@ -514,20 +518,19 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     tmem_st_x32(tp, pk);
                 }
             }
-            pass_turn(j);
+            turn.pass(j);
             tmem_st_x32(tp + 32, pk + 32);
             tmem_st_wait_all();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bp);
-            if (!ok) { ++j; break; }                               // this tile's turn has been passed on
+            if (!ok) { ++j; break; }                               // this tile's turn has been taken and passed on
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         }
-        if (!ok)
-            for (; j < turns; ++j) pass_turn(j);
+        if (!ok) turn.leave(j);
         // ---- result
         if (ok && nt > 0) {
-            ok = mbar_wait(bpv, (nt - 1) & 1u, abort_flag, kAttnPv, p.wait_cycles);
+            ok = wait(bpv, (nt - 1) & 1u, kAttnPv);
             tc_fence_after();
         }
         if (ok && live[t]) {

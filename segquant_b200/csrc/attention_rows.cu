@@ -142,7 +142,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const int vr = (((lane >> 3) & 1) << 3) | (lane & 7), vc = lane >> 4;
     for (int i = warp; i < blocks; i += 4) {
         const int s = i % ST;
-        if (!mbar_wait(smem_u32(&bar_full[s]), (i / ST) & 1u, abort_flag, kRowsFull, p.wait_cycles)) break;
+        if (!mbar_wait_warp(smem_u32(&bar_full[s]), (i / ST) & 1u, abort_flag, kRowsFull, p.wait_cycles)) break;
         const uint32_t ks = sbase + s * 2 * C::kTile, vs = ks + C::kTile;
         const int key0 = k_lo + i * kRowsKeys;
         const int valid = T0.kv_len - key0;

@@ -90,6 +90,26 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
 }
 
+// The same wait by all lanes of a warp that has to stay whole behind it (warp-wide instructions, named barriers): either all of them
+// give up or none.  Lanes give up where all 32 arrive at it together.  A part of the warp there means that the other lanes have seen
+// the phase complete, and goes on with them.  (A vote behind every wait of the attention's softmax warps was measured at 332 -> 340 us
+// for 4429 tokens, 24 heads, two samples; nothing of this lies on the way of a wait that succeeds.)
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code, long long limit) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+#pragma unroll 1
+    for (uint32_t it = 1;; ++it) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((it & 1023u) == 0u && (*abort_flag || clock64() - t0 > limit)) {
+            if (__activemask() != 0xffffffffu) return true;
+            atomicCAS(&g_wait_status, 0ull, (static_cast<unsigned long long>(blockIdx.x) << 8) | static_cast<unsigned>(code));
+            *abort_flag = 1;
+            __threadfence_block();
+            return false;
+        }
+    }
+}
+
 // The same test without a wait, and the record of a wait that gave up, for a thread that watches several barriers.
 __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
     uint32_t done;
