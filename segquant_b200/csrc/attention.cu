@@ -21,9 +21,13 @@
 // 2^(c (m_old - m_new)) when the maximum grows.  O lives in tensor memory and is only rescaled when a row's maximum has
 // grown by more than 2^8 since the last time (every p then stays below 2^8, well inside fp32 sums and fp16 p); the result
 // does not depend on it, the same m is used for p, l and O.  p is rounded once to the 16-bit input type for the second
-// product (half a step, 2^-9 for bf16 and 2^-12 for fp16, of each term); S, l, O and the statistics stay fp32.
+// product (half a step, 2^-8 for bf16 and 2^-11 for fp16, of each term); S, l, O and the statistics stay fp32.  fp16 has no more
+// than steps of 2^-24 below 2^-14, where many keys of small weight beside a strong one would lose theirs, so p, l and O of fp16
+// calls are carried 2^7 times as large (p stays below 2^15): half a step is then at most 2^-32 of the row's largest p.
 #include <cuda.h>
 #include <cudaTypedefs.h>
+
+#include <type_traits>
 
 #include "attention.cuh"
 #include "attention_turns.cuh"
@@ -44,6 +48,9 @@ constexpr int kAttnThreads = 384;
 // 24 heads of 64, two samples: none 361 us, one of eight 335, one of six 332, one of four 347 (the other pipes and the issue
 // slots fill up); 128 wide heads do not care (507, 505, 504, 507 us at 12288 causal tokens).
 constexpr int kPoly = 1, kPolyOf = 6;
+// Power of two that p, l and O are carried up by (see above; what is left of fp16's 2^16 above the 2^8 that a maximum may have grown).
+template <typename T>
+constexpr float kUp = std::is_same<T, __half>::value ? 7.0f : 0.0f;
 constexpr int kWarpMma = 9;         // and the next one with heads up to 64 wide
 constexpr int kAttnRows = 128;       // rows of a sub-tile = tensor-memory lanes
 constexpr int kAttnKeys = 128;       // keys of a tile
@@ -499,7 +506,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             }
             turn.take(j);
             const float mc = m_ref == -INFINITY ? 0.0f : m_ref * c;
-            const float2 c2 = make_float2(c, c), mc2 = make_float2(-mc, -mc);
+            const float off = kUp<T> != 0.0f ? kUp<T> - mc : -mc;
+            const float2 c2 = make_float2(c, c), mc2 = make_float2(off, off);
             float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
             uint32_t pk[64];
 #pragma unroll
@@ -536,7 +544,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (ok && live[t]) {
             const bool empty = m_ref == -INFINITY && l == l;     // no key seen
             const float inv = empty ? 0.0f : 1.0f / l;
-            const float lse2 = empty ? -INFINITY : m_ref * c + log2f(l);
+            const float lse2 = empty ? -INFINITY : m_ref * c + (log2f(l) - kUp<T>);
             const long long token = static_cast<long long>(T0.b) * (p.q_off ? 0 : p.Tq) + T0.q_base + tok;
             const long long r = token * p.Hq + head;
             if (p.splits > 1) {

@@ -12,6 +12,8 @@
 // the two launches and one round trip to memory each are most.
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "attention.cuh"
 #include "ptx.cuh"
 
@@ -20,6 +22,11 @@ namespace sq {
 constexpr int kRowsThreads = 128;
 constexpr int kRowsKeys = 32;        // keys of a block
 enum RowsWait : int { kRowsFull = 30 };
+// Weights (at most 1) are rounded once to the 16-bit type for the product with v, half a step (2^-8 in bf16, 2^-11 in fp16) of each
+// term.  fp16 has no more than steps of 2^-24 below 2^-14, where many keys of small weight beside a strong one would lose theirs:
+// its weights go in 2^14 times as large, and half a step is at most 2^-39 of the largest.
+template <typename T>
+constexpr float kRowsUp = std::is_same<T, __half>::value ? 16384.0f : 1.0f;
 
 template <int DP>
 struct RowsCfg {
@@ -202,8 +209,8 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 e[c] = ex2(sa[n][c] - ms[c >> 1]);
                 l[c >> 1] += e[c];
             }
-            pf[n >> 1][2 * (n & 1)] = pack2<T>(e[0], e[1]);
-            pf[n >> 1][2 * (n & 1) + 1] = pack2<T>(e[2], e[3]);
+            pf[n >> 1][2 * (n & 1)] = pack2<T>(e[0] * kRowsUp<T>, e[1] * kRowsUp<T>);
+            pf[n >> 1][2 * (n & 1) + 1] = pack2<T>(e[2] * kRowsUp<T>, e[3] * kRowsUp<T>);
         }
 #pragma unroll
         for (int k = 0; k < kRowsKeys / 16; ++k) {
@@ -260,7 +267,7 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             acc.x = fmaf(g, v.x, acc.x); acc.y = fmaf(g, v.y, acc.y); acc.z = fmaf(g, v.z, acc.z); acc.w = fmaf(g, v.w, acc.w);
         }
         const bool empty = top == -INFINITY && sum == 0.0f;
-        const float inv = empty ? 0.0f : 1.0f / sum;
+        const float inv = empty ? 0.0f : 1.0f / sum * (1.0f / kRowsUp<T>);
         const long long token = static_cast<long long>(T0.b) * (p.q_off ? 0 : p.Tq) + T0.q_base + tok;
         const long long rr = token * p.Hq + head;
         const float lse2 = empty ? -INFINITY : top + log2f(sum);
