@@ -205,11 +205,11 @@ def load():
     lib.sq_gated_residual.restype = ctypes.c_int
     lib.sq_gated_residual.argtypes = [ctypes.POINTER(GatedResidualArgs), ctypes.c_void_p]
     lib.sq_rotary.restype = ctypes.c_int
-    lib.sq_rotary.argtypes = [ctypes.c_void_p, ctypes.c_void_p]        # the argument block as a structure or as its bytes
+    lib.sq_rotary.argtypes = [ctypes.POINTER(RotaryArgs), ctypes.c_void_p]
     lib.sq_attention.restype = ctypes.c_int
-    lib.sq_attention.argtypes = [ctypes.c_void_p, ctypes.c_void_p]        # the argument block as a structure or as its bytes
+    lib.sq_attention.argtypes = [ctypes.POINTER(AttentionArgs), ctypes.c_void_p]
     lib.sq_attention_scratch_bytes.restype = ctypes.c_int64
-    lib.sq_attention_scratch_bytes.argtypes = [ctypes.c_void_p]
+    lib.sq_attention_scratch_bytes.argtypes = [ctypes.POINTER(AttentionArgs)]
     lib.sq_norm_quantize_act.restype = ctypes.c_int
     lib.sq_norm_quantize_act.argtypes = [ctypes.POINTER(ActQuantArgs), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
                                          ctypes.c_float, ctypes.c_void_p]
@@ -221,13 +221,21 @@ def load():
     lib.sq_unpack_int4.restype = ctypes.c_int
     lib.sq_unpack_int4.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
     lib.sq_gemm.restype = ctypes.c_int
-    lib.sq_gemm.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    lib.sq_gemm.argtypes = [ctypes.POINTER(GemmArgs), ctypes.c_void_p]
     lib.sq_gemm_num_units.restype = ctypes.c_int
     lib.sq_gemm_num_units.argtypes = [ctypes.c_int32, ctypes.POINTER(ctypes.c_int32), ctypes.c_int32]
     lib.sq_seg_linear.restype = ctypes.c_int
     lib.sq_seg_linear.argtypes = [ctypes.POINTER(ActQuantArgs), ctypes.POINTER(GemmArgs), ctypes.c_void_p]
     lib.sq_seg_linear_static.restype = ctypes.c_int
     lib.sq_seg_linear_static.argtypes = [ctypes.POINTER(ActQuantArgs), ctypes.POINTER(GemmArgs), ctypes.c_void_p]
+    # the same entry points for argument blocks that are packed bytes (ops.py)
+    for name in ("sq_gemm", "sq_attention", "sq_rotary"):
+        packed = lib[name]
+        packed.restype, packed.argtypes = ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]
+        setattr(lib, name + "_packed", packed)
+    packed = lib["sq_attention_scratch_bytes"]
+    packed.restype, packed.argtypes = ctypes.c_int64, [ctypes.c_char_p]
+    lib.sq_attention_scratch_bytes_packed = packed
     _LIB = lib
     return lib
 

@@ -320,7 +320,7 @@ def rotary(q, k, positions, axes, *, theta=10000.0, pairing="adjacent", norm_q=N
         a = (q.data_ptr(), 0, out_q.data_ptr(), 0, _dt(q), PAIRINGS[pairing], B, T, qs[-2], 0)
     a = _ROTARY.pack(*a, D, A, struct.pack(f"{A}i", *axes), *qi, *ki, *qo, *ko, positions.data_ptr(), T * A if len(ps) == 3 else 0, A,
                      1 if positions.dtype == torch.float32 else 0, eps, theta, nq, nk)
-    _run(L.load().sq_rotary, "sq_rotary", dev, a)
+    _run(L.load().sq_rotary_packed, "sq_rotary", dev, a)
     if q.numel():
         launch_count += 1
     return out_q, out_k
@@ -446,13 +446,13 @@ def attention(q, k, v, *, causal=False, scale=None, q_offsets=None, kv_offsets=N
                 *strides, q_offsets.data_ptr() if packed else 0, kv_offsets.data_ptr() if packed else 0,
                 q_lens.data_ptr() if q_lens is not None else 0, kv_lens.data_ptr() if kv_lens is not None else 0, scale, 0)
         lib, a = L.load(), _ATTENTION.pack(*head, 0, 0)
-        need = lib.sq_attention_scratch_bytes(a)
+        need = lib.sq_attention_scratch_bytes_packed(a)
         if need < 0:
             L.check(need, "sq_attention_scratch_bytes")
         if need:
             scratch = q.new_empty(need, dtype=torch.uint8)
             a = _ATTENTION.pack(*head, scratch.data_ptr(), need)
-        _run(lib.sq_attention, "sq_attention", dev, a)
+        _run(lib.sq_attention_packed, "sq_attention", dev, a)
         launch_count += 2 if need else 1
     return (out, lse) if return_lse else out
 
@@ -554,7 +554,7 @@ def gemm(kind, xq, wq, N, bounds, sx, sw, *, xq_neg=None, sx_neg=None, per_token
         sw.data_ptr(), *sw_strides,
         bias.data_ptr() if bias is not None else 0, _dt(bias) if bias is not None else 0, 0, 0,
         y.data_ptr(), y_bs, y_rs, acc.data_ptr() if acc is not None else 0, n_peers, 0, *peers, int(prs), int(pco))
-    _run(L.load().sq_gemm, "sq_gemm", xq.get_device(), a)
+    _run(L.load().sq_gemm_packed, "sq_gemm", xq.get_device(), a)
     launch_count += 1
     return (y, acc) if want_acc else y
 
