@@ -527,6 +527,9 @@ def gemm(kind, xq, wq, N, bounds, sx, sw, *, xq_neg=None, sx_neg=None, per_token
         raise TypeError("weight scales must be float32 or bfloat16")
     if S > L.SQ_MAX_SEGS:
         raise L.SegQuantError(L.SQ_ERR_INVALID_ARG, f"at most {L.SQ_MAX_SEGS} segments per call, got {S}")
+    bounds = [int(b) for b in bounds]
+    if any(not 0 <= b < 1 << 31 for b in bounds):
+        raise L.SegQuantError(L.SQ_ERR_INVALID_ARG, f"segment bounds must be non-negative 32-bit numbers: {bounds}")
     Kw = (bounds[1] - bounds[0]) if w_seg_as_batch else K
     w_row = Kw // 2 if w4 else Kw
     sx_strides = (S * M, M, 1) if per_token else (S, 1, 0)
