@@ -12,6 +12,7 @@ import ctypes
 import struct
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib as L
 
@@ -278,8 +279,10 @@ def rotary(q, k, positions, axes, *, theta=10000.0, pairing="adjacent", norm_q=N
     dev = q.get_device()
     if not q.is_cuda or not positions.is_cuda or not (k is None or k.is_cuda):
         _need_cuda(q, k, positions)
-    if q.requires_grad or (k is not None and k.requires_grad) or (norm_q is not None and norm_q.requires_grad) or (norm_k is not None and norm_k.requires_grad):
-        _no_grad(q, k, norm_q, norm_k)
+    if q.requires_grad or positions.requires_grad or any(t is not None and t.requires_grad for t in (k, norm_q, norm_k)):
+        _no_grad(q, k, positions, norm_q, norm_k)
+    if _forward_ad._current_level >= 0:
+        _no_tangent(q, k, positions, norm_q, norm_k, out_q, out_k)
     if pairing not in PAIRINGS:
         raise ValueError(f"pairing must be one of {list(PAIRINGS)}")
     qs, dt, A = q.shape, q.dtype, len(axes)
@@ -350,6 +353,12 @@ def _no_grad(*tensors):
         raise RuntimeError("segquant_b200: this operator has no backward pass; detach its inputs or run it under torch.no_grad()")
 
 
+def _no_tangent(*tensors):
+    """Called inside a forward-mode level only: elsewhere no tensor has a tangent."""
+    if any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("segquant_b200: this operator has no derivative; its inputs may not carry tangents")
+
+
 def _tma_view(t):
     """t itself where the kernel can read it in place (last dimension contiguous, other strides positive multiples of 16
     bytes, 16-byte aligned), else a contiguous copy."""
@@ -385,6 +394,8 @@ def attention(q, k, v, *, causal=False, scale=None, q_offsets=None, kv_offsets=N
         _need_cuda(q, k, v)
     if q.requires_grad or k.requires_grad or v.requires_grad:
         _no_grad(q, k, v)
+    if _forward_ad._current_level >= 0:
+        _no_tangent(q, k, v, out)
     packed = q_offsets is not None
     if kv_offsets is not None and not packed:
         raise ValueError("attention: kv_offsets needs q_offsets")
