@@ -9,6 +9,7 @@ The two functions at the bottom keep the tensor contract of the reference's pybi
 layer forward that SegmentLinear uses.
 """
 import ctypes
+import functools
 import struct
 
 import torch
@@ -261,6 +262,58 @@ def quantize_act_dynamic(x, bounds, out_kind=L.SQ_Q_INT8, dual=False, smooth=Non
 
 
 # ---------------------------------------------------------------------------------------------
+# outputs that are given
+# ---------------------------------------------------------------------------------------------
+def _meets(r, width, dims, moved):
+    """Whether r + sum d_i stride_i lies within (-width, width) for some d; dims: (stride, least d, greatest d) from the largest
+    stride on.  Exact: d is tried as far as the smaller strides can make up for it, once or twice a dimension in a nested layout.
+    moved false: d = 0 does not count."""
+    if not dims:
+        return moved and -width < r < width
+    (s, lo, hi), rest = dims[0], dims[1:]
+    least, most = sum(t * l for t, l, _ in rest), sum(t * h for t, _, h in rest)
+    first, last = max(lo, (-width - most - r) // s + 1), min(hi, -((r + least - width) // s) - 1)
+    return any(_meets(r + d * s, width, rest, moved or d != 0) for d in range(first, last + 1))
+
+
+@functools.lru_cache(maxsize=1024)
+def _layout_overlaps_itself(shape, stride):
+    dims = [(s, 1 - n, n - 1) for n, s in zip(shape[:-1], stride) if n > 1]
+    return any(s == 0 for s, _, _ in dims) or _meets(0, shape[-1], sorted(dims, reverse=True), False)
+
+
+def _overlaps_itself(t):
+    return not t.is_contiguous() and t.numel() > 0 and _layout_overlaps_itself(t.shape, t.stride())
+
+
+@functools.lru_cache(maxsize=1024)
+def _layouts_overlap(gap, es, shape_a, stride_a, shape_b, stride_b):
+    reach = lambda shape, stride: es * (sum((n - 1) * s for n, s in zip(shape, stride)) + 1)  # noqa: E731
+    if gap >= reach(shape_b, stride_b) or -gap >= reach(shape_a, stride_a):
+        return False
+    dims = []
+    for na, sa, nb, sb in zip(shape_a[:-1], stride_a, shape_b[:-1], stride_b):
+        if na == 1 and nb == 1:
+            continue
+        if na > 1 and nb > 1 and sa != sb:
+            return False
+        s = sa if na > 1 else sb
+        if s:
+            dims.append((es * s, 1 - nb, na - 1))
+    return _meets(gap, es * shape_a[-1], sorted(dims, reverse=True), True)
+
+
+def _overlap(a, b):
+    """Whether a and b (one dtype, last dimensions contiguous and as wide) share an element: exactly where their strides are the same, else
+    where they start at the same address or lie apart as a whole.  A matter of the layouts and the distance between the two, which
+    a program's calls repeat: worked out once for each (13 us in a buffer of q | k | v)."""
+    if not a.numel() or not b.numel():
+        return False
+    gap = a.data_ptr() - b.data_ptr()
+    return gap == 0 or (abs(gap) < 1 << 40 and _layouts_overlap(gap, a.element_size(), a.shape, a.stride(), b.shape, b.stride()))
+
+
+# ---------------------------------------------------------------------------------------------
 # rotary positions
 # ---------------------------------------------------------------------------------------------
 PAIRINGS = {"adjacent": L.SQ_ROTARY_ADJACENT, "halves": L.SQ_ROTARY_HALVES}
@@ -312,9 +365,13 @@ def rotary(q, k, positions, axes, *, theta=10000.0, pairing="adjacent", norm_q=N
         if norm_k is not None:
             norm_k = norm_k.contiguous()
             nk = norm_k.data_ptr()
+    given = out_q is not None, out_k is not None and k is not None
     q, out_q, qi, qo = _rotary_pair(q, out_q, "q")
     if k is not None:
         k, out_k, ki, ko = _rotary_pair(k, out_k, "k")
+        if (given[0] and _overlap(out_q, k)) or (given[1] and not (out_k is k and out_q is q) and _overlap(out_k, q)) or \
+                (given[0] and given[1] and not (out_k is k or out_q is q) and _overlap(out_q, out_k)):
+            raise ValueError("rotary: an output overlaps the other tensor")
         a = (q.data_ptr(), k.data_ptr(), out_q.data_ptr(), out_k.data_ptr(), _dt(q), PAIRINGS[pairing], B, T, qs[-2], k.shape[-2])
     elif out_k is not None:
         raise ValueError("rotary: out_k without k")
@@ -339,8 +396,12 @@ def _rotary_pair(x, out, name):
         xs = x.stride()
     if out is None:
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
-    elif out is not x and (out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1):
-        raise ValueError(f"rotary: out_{name} must have {name}'s shape, dtype and device and a contiguous last dimension")
+    else:
+        if out is not x and (out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or out.stride(-1) != 1):
+            raise ValueError(f"rotary: out_{name} must have {name}'s shape, dtype and device and a contiguous last dimension")
+        same = out is x or (out.data_ptr() == x.data_ptr() and all(n == 1 or a == b for n, a, b in zip(x.shape, out.stride(), xs)))
+        if _overlaps_itself(out) or (not same and _overlap(out, x)):
+            raise ValueError(f"rotary: out_{name} overlaps itself, or {name} without being the same elements")
     os = out.stride()
     return (x, out, xs[:3], os[:3]) if len(xs) == 4 else (x, out, (0, xs[0], xs[1]), (0, os[0], os[1]))
 
@@ -439,6 +500,8 @@ def attention(q, k, v, *, causal=False, scale=None, q_offsets=None, kv_offsets=N
         if out.shape != qs or out.dtype != dt or out.device != q.device or _tma_view(out) is not out:
             raise ValueError("attention: out must have q's shape, dtype and device, a contiguous last dimension, and strides and address in "
                              "multiples of 16 bytes")
+        if _overlaps_itself(out) or _overlap(out, q) or _overlap(out, k) or _overlap(out, v):
+            raise ValueError("attention: out overlaps itself or an input")
     lse = torch.full(qs[:-1], float("-inf"), dtype=torch.float32, device=q.device) if return_lse else None
     if packed and B == 0:
         if fill_rest:
