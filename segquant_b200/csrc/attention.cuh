@@ -25,10 +25,8 @@ struct AttnParams {
     int splits;              // parts that the keys of a tile are cut into
     int part_keys;           // rows kernel: keys of a part (the large kernel cuts what a tile sees into equal parts)
     float scale_log2;        // scale * log2(e)
-    long long q_bs, q_ts, q_hs, k_bs, k_ts, k_hs, v_bs, v_ts, v_hs, o_bs, o_ts, o_hs;   // element strides: batch, token, head
+    long long q_bs, q_ts, q_hs, o_bs, o_ts, o_hs;   // element strides: batch, token, head (k and v come as tensor maps)
     const void* q;
-    const void* k;
-    const void* v;
     void* out;
     float* lse;              // [batch * Tq (packed: Tq), Hq] natural logarithm of the row sums, or NULL
     float* part_o;           // splits > 1: [splits][tokens * Hq][D], each part normalised by itself
@@ -130,11 +128,6 @@ __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float lg2(float x) {
-    float y;
-    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {      // NaN counts as absent, as in fmaxf

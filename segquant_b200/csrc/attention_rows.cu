@@ -41,12 +41,6 @@ struct RowsCfg {
     static constexpr uint32_t kSmem = 1024 + kRing;
 };
 
-__device__ __forceinline__ void rows_tma(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
-        : "memory");
-}
 __device__ __forceinline__ void ldsm(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -109,8 +103,8 @@ attention_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         const uint32_t bar = smem_u32(&bar_full[s]), dst = sbase + s * 2 * C::kTile;
         const int tok = T0.kv_base + k_lo + i * kRowsKeys;
         mbar_arrive_expect_tx(bar, 2 * C::kTile);
-        for (int h = 0; h < DP / 64; ++h) rows_tma(dst + h * C::kHalf, &map_k, h * 64, kvh, tok, T0.b, bar);
-        for (int h = 0; h < DP / 64; ++h) rows_tma(dst + C::kTile + h * C::kHalf, &map_v, h * 64, kvh, tok, T0.b, bar);
+        for (int h = 0; h < DP / 64; ++h) tma_load_4d(dst + h * C::kHalf, &map_k, h * 64, kvh, tok, T0.b, bar);
+        for (int h = 0; h < DP / 64; ++h) tma_load_4d(dst + C::kTile + h * C::kHalf, &map_v, h * 64, kvh, tok, T0.b, bar);
     };
     if (threadIdx.x == 0)
         for (int i = 0; i < ST && i < blocks; ++i) order(i);
