@@ -332,7 +332,8 @@ def rotary(q, k, positions, axes, *, theta=10000.0, pairing="adjacent", norm_q=N
     dev = q.get_device()
     if not q.is_cuda or not positions.is_cuda or not (k is None or k.is_cuda):
         _need_cuda(q, k, positions)
-    if q.requires_grad or positions.requires_grad or any(t is not None and t.requires_grad for t in (k, norm_q, norm_k)):
+    if q.requires_grad or positions.requires_grad or (k is not None and k.requires_grad) or (norm_q is not None and norm_q.requires_grad) or \
+            (norm_k is not None and norm_k.requires_grad):
         _no_grad(q, k, positions, norm_q, norm_k)
     if _forward_ad._current_level >= 0:
         _no_tangent(q, k, positions, norm_q, norm_k, out_q, out_k)
@@ -601,9 +602,11 @@ def gemm(kind, xq, wq, N, bounds, sx, sw, *, xq_neg=None, sx_neg=None, per_token
         raise TypeError("weight scales must be float32 or bfloat16")
     if S > L.SQ_MAX_SEGS:
         raise L.SegQuantError(L.SQ_ERR_INVALID_ARG, f"at most {L.SQ_MAX_SEGS} segments per call, got {S}")
-    bounds = [int(b) for b in bounds]
-    if any(not 0 <= b < 1 << 31 for b in bounds):
-        raise L.SegQuantError(L.SQ_ERR_INVALID_ARG, f"segment bounds must be non-negative 32-bit numbers: {bounds}")
+    bounds = [*map(int, bounds)]
+    try:
+        packed_bounds = struct.pack(f"{S + 1}i", *bounds)
+    except struct.error:
+        raise L.SegQuantError(L.SQ_ERR_INVALID_ARG, f"segment bounds past 32 bits: {bounds}") from None
     Kw = (bounds[1] - bounds[0]) if w_seg_as_batch else K
     w_row = Kw // 2 if w4 else Kw
     sx_strides = (S * M, M, 1) if per_token else (S, 1, 0)
@@ -625,7 +628,7 @@ def gemm(kind, xq, wq, N, bounds, sx, sw, *, xq_neg=None, sx_neg=None, per_token
         kind, _DT[out_dtype], batch, M, N, K,
         xq.data_ptr(), xq_neg.data_ptr() if xq_neg is not None else 0, M * K if (x_batched and Bx > 1) else 0, K,
         wq.data_ptr(), N * w_row if Bw > 1 else 0, w_row, 1 if w_seg_as_batch else 0,
-        S, struct.pack(f"{S + 1}i", *bounds), int(group_size or 0), 1 if sw.dtype == torch.bfloat16 else 0,
+        S, packed_bounds, int(group_size or 0), 1 if sw.dtype == torch.bfloat16 else 0,
         sx.data_ptr(), sx_neg.data_ptr() if sx_neg is not None else 0,
         sx_strides[0] if sx_batch_stride is None else sx_batch_stride, sx_strides[1], sx_strides[2],
         sw.data_ptr(), *sw_strides,
