@@ -213,6 +213,8 @@ int sq_gated_residual(const sq_gated_residual_args* args, sq_stream_t stream);
  * queries of a prompt's next piece, or a single new token, continue the keys that are there.  A query that sees no key gets 0
  * (lse: -inf).  Keys outside a sequence never reach its rows, whatever bits they hold; a NaN or infinity in a v row that
  * another query of the sequence sees may also reach earlier queries (0 * inf), as in the product it stands for.
+ * The softmax weights are rounded once to the dtype for the product with v (half a step, 2^-8 of a weight in bf16 and 2^-11 in fp16, there
+ * down to 2^-32 of the row's largest weight).
  * Rows of out (and lse) that belong to no sequence are left alone, or set like rows that see no key with fill_rest.
  * D: a multiple of 8 up to SQ_ATTENTION_MAX_D, contiguous; strides in elements, multiples of 8 and positive; pointers 16-byte
  * aligned.  out must not overlap q, k or v.  lse_dev: NULL or float [tokens, Hq], log of the row sums (natural).
@@ -252,7 +254,8 @@ int sq_attention(const sq_attention_args* args, sq_stream_t stream);
 int64_t sq_attention_scratch_bytes(const sq_attention_args* args);
 
 /* ---- rotary positions (no counterpart in the reference) -------------------------------------------------------------
- * The D columns of a head are cut into one block of axes[a] columns per axis; columns behind the last block are not rotated.
+ * The D columns of a head are cut into one block of axes[a] columns per axis; columns behind the last block are not rotated
+ * (without norm weights they keep their bits, but for the bits of a NaN).
  * Pair i of axis a turns by  positions[b, t, a] * theta^(-2 i / axes[a])  (reduced in fp64):
  *   (y0, y1) -> (y0 cos - y1 sin, y0 sin + y1 cos)
  * with y = x, or with the norm weights y = x * rsqrt(mean(x^2) + eps) * weight over the head's D columns first.  Arithmetic in
@@ -338,6 +341,10 @@ int sq_unpack_int4(const void* packed_dev, void* out_dev, int64_t numel, sq_stre
  * If w_seg_as_batch != 0 the weights of segment s are a separate [N, seg_len] matrix found at
  * batch index s of wq (the reference's packed layout (segments, N*seg/2),
  * segquant/layers/segment_tensor_manager.py:56-66) and `batch` must be 1.
+ *
+ * W4A8 with batch 1, M <= 8, K <= 65536 and sides * M * (K + 16) <= 99328 (sides: 2 with DualScale; 8 rows: K <= 12400, DualScale
+ * 6192) runs on a weight-streaming kernel with the same results, unless it has peer outputs, an accumulator dump, weights by segment
+ * or over 512 units in several segments; anything else on 128-row tiles, which a few rows leave mostly empty (several times slower).
  *
  * acc_dump_dev (NULL in production): if set, unit u's raw accumulator words are also written to
  * acc_dump_dev[((b*units + u)*sides + side)*M*N + m*N + n] (int32, or fp32 bits for e4m3);

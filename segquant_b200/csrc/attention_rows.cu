@@ -6,10 +6,9 @@
 // each of four warps works on key blocks of its own (32 keys, in turn), with mma.sync m16n8k16 from registers to registers: S
 // of a block is in the layout that the product with v wants its first operand in.  Loads go through a ring of blocks that the
 // warps share; the warp that is done with a block's slot orders the next block into it, so nothing but the loads is ever
-// waited for.  The warps' maxima, sums and outputs are joined in shared memory, the parts of a row by a second kernel that is
-// launched behind this one and is already resident when it ends.  32 caches of 4000 to 16001 keys, 8 key heads of 128, 32
-// query heads: 182 us = 6.0 TB/s of the 1.1 GB (copy bandwidth 6.55); one cache of 1531 keys, 8 heads of 64: 9 to 10 us, of which
-// the two launches and one round trip to memory each are most.
+// waited for.  The warps' maxima, sums and outputs are joined in shared memory, the parts of a row by a second kernel behind this
+// one.  32 caches of 369 to 16001 keys, 8 key heads of 128, 32 query heads: 182 us = 6.0 TB/s of the 1.1 GB (copy bandwidth 6.55);
+// one cache of 1531 keys, 8 heads of 64: 9 to 10 us, of which the two launches and one round trip to memory each are most.
 #include <cuda.h>
 
 #include <type_traits>

@@ -370,7 +370,8 @@ int gemm(const sq_gemm_args* a, cudaStream_t st) {
         SQ_REQUIRE(a->bias_dtype == SQ_F32 || a->bias_dtype == SQ_F16 || a->bias_dtype == SQ_BF16, SQ_ERR_INVALID_ARG,
                    "sq_gemm: unknown bias_dtype %d", a->bias_dtype);
     p.wait_cycles = overrides().wait_cycles;
-    // a handful of rows: stream the weights once on the CUDA cores instead of padding 128-row tensor-core tiles
+    // a handful of rows: stream the weights once instead of padding 128-row tiles (8-bit weights: dot products on the CUDA cores;
+    // int4: mma.sync)
     if (gemv_applies(a, dual)) return launch_gemv(p, a, dual, st);
     if (gemv_w4_applies(a, dual, units)) return launch_gemv_w4(p, a, dual, st);
     // Fused all-gather: stores to peers should be whole 128-byte lines ([16 rows x 128 bytes] boxes, see store_output).

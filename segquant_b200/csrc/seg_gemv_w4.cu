@@ -12,8 +12,9 @@
 // memory with the even and the odd bytes of every 8 columns side by side.  An output lives in one lane from the first unit to
 // the last, so the fp32 sum over the units runs in registers.
 //
-// 16384 x 12288, groups of 128, 4 rows (98 MB of weights, floor 16 us): 42 us, 147 us on the 128-row tiles.  7 warps an SM walk
-// 96 blocks each, some 150 instructions a block, and that chain bounds it (without groups, 28 us).  Measured and not kept:
+// 16384 x 12288, groups of 128, 4 rows (101 MB of weights and 6 MB of scales, floor 16.4 us): 42 us, 147 us on the 128-row tiles; 7
+// warps an SM walk 96 blocks each, some 150 instructions a block (without groups, 29 us).  What bounds it is not established: memory,
+// issue slots (33 %) and the tensor pipe (7 %) are far from full.  Measured and not kept:
 // dot products on the ALUs (dp4a) 72 us; two blocks a step 51; scales through the ring 43; closing a unit a block later 43;
 // tiles of 8 columns on twice the warps 48; three warps to a tile that exchange their integer sums 42 to 52.
 #include <cstdlib>
@@ -264,7 +265,11 @@ __global__ void __launch_bounds__(kW4Warps * 32, 1) seg_gemv_w4_kernel(const __g
 
 static long long w4_x_bytes(const sq_gemm_args* a, bool dual) { return (dual ? 2 : 1) * a->M * (a->K + 16); }
 
-// True when the skinny path serves this problem (the caller has validated the arguments).
+// True when the skinny path serves this problem (the caller has validated the arguments).  Against the 128-row tiles it was faster
+// at every one of 668 sizes that it serves (1, 2, 4, 8 rows; 16 to 16384 columns; K 256 to 65536; no groups, 32, 64, 128; one side or two):
+// 1.8 to 9.4 times.  16384 x 12288, us on this path / on tiles, 1 and 8 rows: no groups 24 / 75 and 35 / 72, groups of 128 39 / 146 and
+// 49 / 147, of 64 75 / 274 and 84 / 273, of 32 113 / 531 and 123 / 529.  The rows have to fit shared memory: 8 rows up to K = 12400, with
+// two sides 6192; behind that a call is on tiles again (8 rows, two sides, groups of 128, 16384 x 12288: 328 us; 4 rows fit and take 57).
 bool gemv_w4_applies(const sq_gemm_args* a, bool dual, int units) {
     if (a->kind != SQ_GEMM_W4A8 || a->batch != 1 || a->M > kW4MaxRows || a->acc_dump_dev != nullptr || a->num_peer_outputs != 0 || a->w_seg_as_batch)
         return false;

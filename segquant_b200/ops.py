@@ -327,7 +327,7 @@ def rotary(q, k, positions, axes, *, theta=10000.0, pairing="adjacent", norm_q=N
     position * theta ** (-2 i / axes[a]); pairing "adjacent" pairs columns (2i, 2i + 1) of a block, "halves" (i, i + width / 2).
     norm_q / norm_k: (D,) weights of the heads' RMS normalisation in front of the rotation, in q's dtype, both or neither.
     float32, float16 and bfloat16, D up to 256; arithmetic in fp32 (angles in fp64), rounded once.  out_q / out_k may be q / k
-    themselves.  Returns (q, k) rotated; (q, None) without k."""
+    themselves and overlap nothing else, themselves included.  No derivatives: inputs that want any are refused.  Returns (q, k) rotated; (q, None) without k."""
     global launch_count
     dev = q.get_device()
     if not q.is_cuda or not positions.is_cuda or not (k is None or k.is_cuda):
@@ -449,7 +449,8 @@ def attention(q, k, v, *, causal=False, scale=None, q_offsets=None, kv_offsets=N
 
     causal: query i of a sequence sees its keys below i + 1 + kv_len - q_len, so its last query sees its last key.  A
     query that sees no key gets 0 (lse -inf).  Rows that belong to no sequence are 0 in a new result and left alone in
-    `out`, which has q's shape and dtype, D contiguous, strides and address multiples of 16 bytes, and overlaps no input.
+    `out`, which has q's shape and dtype, D contiguous, strides and address multiples of 16 bytes, and overlaps neither itself nor an input.
+    No derivatives: inputs that want any are refused.
     return_lse: also the float32 logarithm of the row sums, (B, Tq, Hq) or (Nq, Hq)."""
     global launch_count
     if not (q.is_cuda and k.is_cuda and v.is_cuda):
